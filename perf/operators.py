@@ -62,7 +62,7 @@ def listed():
         # The recogniser's qkv layer for one time step.
         {"name": "q4 one step f32", "op": "q4", "x": "f32", "y": "f32", "rows": 1, "k": 120, "n": 360, "group": 32, "zeros": False},
         # The class head for sixteen time steps, over the dictionary's 18 710 classes.
-        {"name": "q4 head f16", "op": "q4", "x": "f16", "y": "f32", "rows": 16, "k": 120, "n": 18710, "group": 40, "zeros": True},
+        {"name": "q4 head f16", "op": "q4", "x": "f16", "y": "f32", "rows": 16, "k": 120, "n": 18710, "group": 32, "zeros": True},
         # A wide feed-forward layer for one step: the bandwidth-bound end.
         {"name": "q4 wide bf16", "op": "q4", "x": "bf16", "y": "bf16", "rows": 1, "k": 8192, "n": 28672, "group": 128, "zeros": False},
         # A batch of steps behind the norm's 8-bit rows.
@@ -84,7 +84,7 @@ def draw(rng):
     if op == "q4":
         x = rng.choice(["f32", "f16", "bf16", "e4m3"])
         return {"op": "q4", "x": x, "y": rng.choice(["f32", "f16", "bf16"]), "rows": _log(rng, 1, 32),
-                "k": _log(rng, 64, 8192), "n": _log(rng, 64, 28672), "group": rng.choice([32, 40, 64, 128]),
+                "k": _log(rng, 64, 8192), "n": _log(rng, 64, 28672), "group": rng.choice([32, 64, 128]),
                 "zeros": rng.random() < 0.5}
     kv_heads = rng.choice([1, 2, 4, 8])
     share = rng.choice([1, 1, 2, 4])
