@@ -173,6 +173,109 @@ int ppocr_rec_input_hwc(const uint8_t *crop, size_t width, size_t height, float 
 int ppocr_db_mask(const float *prob, size_t pixels, float thresh, uint8_t *mask, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Transformer-block operators over device buffers the caller owns, beside
+ * the plan kinds attention, layernorm and conv 1x1 that a model runs: attention
+ * with a sliding window and sinks, the root-mean-square norm with an 8-bit
+ * output, and the product with 4-bit weights. No counterpart in the
+ * reference (its blocks are full attention, LayerNorm and f32 products).
+ *
+ * Each call is enqueued on `stream` (a cudaStream_t of the current device;
+ * NULL is the default stream), allocates nothing, keeps nothing, needs no
+ * workspace and may run at the same time as any other call, or be captured
+ * in a graph. Buffers are device memory of the current device. The shapes
+ * are read during the call only. Bad arguments return PPOCR_E_ARG and sizes
+ * beyond the stated limits PPOCR_E_SIZE before any launch.
+ * ---------------------------------------------------------------------- */
+
+/* Element types. */
+enum {
+    PPOCR_F32 = 0,
+    PPOCR_F16 = 1,
+    PPOCR_BF16 = 2,
+    PPOCR_E4M3 = 3 /* 8 bits: 4 of exponent, 3 of mantissa, largest 448, no infinities */
+};
+
+/* Sizes of one ppocr_attention_window. Strides are in elements; elements of
+ * one head's row lie side by side. */
+typedef struct {
+    int32_t type;                            /* of q, k, v and out: PPOCR_F32, _F16 or _BF16 */
+    uint32_t lanes, heads, kv_heads;         /* heads a multiple of kv_heads: head h reads key head h / (heads / kv_heads) */
+    uint32_t head_dim;                       /* 1 to 128 */
+    int32_t left, right;                     /* keys seen before and behind the query's own; -1: no limit */
+    uint32_t sinks;                          /* a lane's first keys, seen however far back they are */
+    float scale;                             /* of the scores */
+    uint32_t max_q, max_k;                   /* about the longest lane's queries and keys (0: unknown); they size
+                                                the launch, never the result */
+    uint64_t q_rows, kv_rows;                /* rows q and out, and k and v, hold (at most 2^30) */
+    uint64_t q_row, q_head, k_row, k_head;   /* strides from row to row and head to head */
+    uint64_t v_row, v_head, out_row, out_head;
+} ppocr_attention_shape;
+
+/* Attention with a sliding window and sinks over packed lanes (the plan kind
+ * `attention` sees every key). Lane b's queries are rows q_offsets[b] to
+ * q_offsets[b + 1] - 1 of q and out, its keys the k_len[b] rows of k and v from
+ * k_begin[b] on (both NULL: the queries' own rows). Its queries stand at the
+ * end of its keys: query i of nq at position p = i + nk - nq, so a step's one
+ * query behind a cache of nk - 1 keys and its own is the last, and a whole
+ * line's queries are their keys. Query i sees key j when
+ *     j <= p + right and (j >= p - left or j < sinks),
+ * and out = sum over the keys seen of softmax(scale * q . k) v: zeros when it
+ * sees none (nk = 0, or before the first key when nq > nk). Keys that a query does not
+ * see never reach its output, whatever they hold. The arrays are in device memory, non-decreasing
+ * in q_offsets (lanes + 1 values); rows outside the tensors are cut off, and
+ * rows of out in no lane stay as they are. Sums and softmax are f32 (f32 products in
+ * 3xTF32; f16 and bf16 weights rounded to the type for the second product).
+ * out may not overlap q, k or v. */
+int ppocr_attention_window(const ppocr_attention_shape *shape, const void *q, const void *k, const void *v, void *out,
+                           const int64_t *q_offsets, const int64_t *k_begin, const int32_t *k_len, void *stream);
+
+/* Sizes of one ppocr_rms_norm_e4m3. Row strides are in elements, 0 meaning
+ * rows side by side. */
+typedef struct {
+    int32_t type;      /* of x, residual and sum: PPOCR_F32, _F16 or _BF16 */
+    uint32_t channels; /* 1 to 32768 */
+    uint32_t group;    /* channels that share a scale: 32, 64 or 128; 0: the row */
+    float eps;
+    uint64_t rows;
+    uint64_t x_row, residual_row, sum_row, y_row;
+} ppocr_rms_norm_shape;
+
+/* The residual's addition, a root-mean-square norm and its 8-bit output:
+ *     s = x + residual,  n = s / sqrt(mean(s^2) + eps) * gamma,
+ *     scale = max |n| over the group / 448,  y = e4m3(n / scale),
+ * in f32 until the last rounding. s is written to `sum` rounded to the type
+ * (NULL: not written; x or residual themselves: updated in place) and
+ * ceil(channels / group) scales a row to `scales`. residual may be NULL
+ * (s = x). A group of zeros has scale 0 and zeros; one with a NaN, scale NaN and
+ * NaNs. Rows are independent. y and scales overlap nothing else. */
+int ppocr_rms_norm_e4m3(const ppocr_rms_norm_shape *shape, const void *x, const void *residual, const float *gamma,
+                        void *sum, uint8_t *y, float *scales, void *stream);
+
+/* Sizes of one ppocr_matvec_q4. Row strides are in elements (w_row in
+ * bytes), 0 meaning rows side by side. */
+typedef struct {
+    int32_t x_type;     /* PPOCR_F32, _F16, _BF16 or _E4M3 */
+    int32_t y_type;     /* PPOCR_F32, _F16 or _BF16 */
+    int32_t scale_type; /* PPOCR_F32, _F16 or _BF16 */
+    uint32_t rows;      /* of x and y: at most 32 */
+    uint32_t k, n;      /* x is rows x k, w n x k, y rows x n */
+    uint32_t group;     /* weights that share a scale: a multiple of 32 */
+    uint32_t x_group;   /* e4m3: `group` when x has a scale a group, 0 when one a row */
+    uint64_t x_row, y_row, w_row;
+} ppocr_matvec_q4_shape;
+
+/* y = x w^T + bias for a few rows of x and 4-bit weights:
+ *     y[m][n] = sum_k x[m][k] (q[n][k] - z[n][k / group]) scales[n][k / group] + bias[n],
+ * two weights q (0 to 15) a byte, the even one in the lower bits, rows of
+ * ceil(k / 2) bytes or more; ceil(k / group) scales and zero points (a byte each, 0 to 15; NULL:
+ * 8) a row; bias f32 or NULL. e4m3 rows of x (ppocr_rms_norm_e4m3's) come with
+ * their x_scales. Every product is exact and every sum f32 (f32 rows of x as
+ * three bf16 parts); y is rounded once. Fastest with w and w_row multiples of
+ * 16 bytes. y overlaps nothing else. */
+int ppocr_matvec_q4(const ppocr_matvec_q4_shape *shape, const void *x, const float *x_scales, const uint8_t *w,
+                    const void *scales, const uint8_t *zeros, const float *bias, void *y, void *stream);
+
+/* ------------------------------------------------------------------------
  * Page reading: the steps around the two networks.
  *
  * The reference's library exposes its page steps as plain functions the

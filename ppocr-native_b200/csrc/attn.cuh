@@ -1,0 +1,328 @@
+// Window attention: the arguments and the warp-level pieces that its kernels
+// share.
+//
+// Lane b has queries i in [0, nq) and keys j in [0, nk); query i stands at
+// key position p = i + nk - nq. It sees key j when
+//     j <= p + right  and  (j >= p - left  or  j < sinks),
+// a negative left or right meaning no limit, and its output is
+//     sum_j softmax_j(scale * q_i . k_j) v_j   over the keys it sees,
+// zero when it sees none. The softmax runs in one pass: a running maximum m
+// and sum l per row in f32, the accumulator scaled by 2^(m_old - m_new)
+// whenever the maximum moves, scores in units of log2 (scale * log2 e).
+#pragma once
+
+#include "block.cuh"
+
+namespace ppocr {
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    void *out;
+    const int64_t *q_offsets, *k_begin;
+    const int32_t *k_len;
+    int64_t q_rows, kv_rows;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
+    int lanes, heads, kv_heads, share, d;
+    int left, right, sinks;  // left, right -1: no limit
+    float scale, scale_log2;
+    int q_bytes, k_bytes, v_bytes;  // widest copy each tensor's rows allow: 16, 4 or 2 bytes
+    int out_vec;                     // 1 when pairs of outputs may be stored together
+};
+
+namespace {
+
+struct Lane {
+    int64_t q0, k0;  // first row of its queries and of its keys
+    int nq, nk;
+};
+
+// A lane's rows, cut to the rows the tensors hold whatever the arrays say.
+__device__ __forceinline__ Lane read_lane(const AttnArgs &a, int b) {
+    Lane l;
+    int64_t q0 = __ldg(a.q_offsets + b), q1 = __ldg(a.q_offsets + b + 1);
+    q0 = q0 < 0 ? 0 : q0 > a.q_rows ? a.q_rows : q0;
+    q1 = q1 < q0 ? q0 : q1 > a.q_rows ? a.q_rows : q1;
+    int64_t k0 = q0, n = q1 - q0;
+    if (a.k_begin) {
+        k0 = __ldg(a.k_begin + b);
+        n = __ldg(a.k_len + b);
+    }
+    k0 = k0 < 0 ? 0 : k0 > a.kv_rows ? a.kv_rows : k0;
+    n = n < 0 ? 0 : n > a.kv_rows - k0 ? a.kv_rows - k0 : n;
+    l.q0 = q0;
+    l.nq = int(q1 - q0);
+    l.k0 = k0;
+    l.nk = int(n);
+    return l;
+}
+
+__device__ __forceinline__ bool sees(const AttnArgs &a, int p, int j) {
+    return (a.right < 0 || j <= p + a.right) && (a.left < 0 || j >= p - a.left || j < a.sinks);
+}
+
+// The key tiles that queries at positions [p0, p1] need: the sinks below the
+// window first, then the window from a multiple of the tile size on.
+struct KeyTiles {
+    int sink_end, lo, hi, n_sink, n;
+    template <int BK>
+    __device__ __forceinline__ void plan(const AttnArgs &a, int p0, int p1, int nk) {
+        hi = a.right < 0 ? nk : min(nk, p1 + a.right + 1);
+        hi = max(hi, 0);
+        lo = a.left < 0 ? 0 : max(0, p0 - a.left);
+        lo = min(lo / BK * BK, hi);
+        sink_end = min(a.sinks, lo);
+        n_sink = (sink_end + BK - 1) / BK;
+        n = n_sink + (hi - lo + BK - 1) / BK;
+    }
+    // tile `it`: its keys are [first, end), fewer than BK at the ends
+    template <int BK>
+    __device__ __forceinline__ int first(int it) const {
+        return it < n_sink ? it * BK : lo + (it - n_sink) * BK;
+    }
+    __device__ __forceinline__ int end(int it) const { return it < n_sink ? sink_end : hi; }
+};
+
+// Rows [0, rows) of a tensor's one head into a shared tile of ROWS rows of
+// STRIDE elements, zeros past `rows` and past d, by `threads` threads.
+template <class T, int ROWS, int DP, int STRIDE, int W>
+__device__ __forceinline__ void load_rows_w(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int tid,
+                                            int threads) {
+    constexpr int E = W / int(sizeof(T)), CPR = DP / E;
+    for (int e = tid; e < ROWS * CPR; e += threads) {
+        const int r = e / CPR, c = e % CPR;
+        const int left = r < rows ? (d - c * E) * int(sizeof(T)) : 0;
+        const int valid = left < 0 ? 0 : left > W ? W : left;
+        const T *from = valid ? src + r * row_stride + c * E : src;
+        const uint32_t to = dst + uint32_t((r * STRIDE + c * E) * int(sizeof(T)));
+        if constexpr (W >= 4) {
+            copy_async<W>(to, from, valid);
+        } else {
+            uint16_t v = 0;
+            if (valid) v = __ldg(reinterpret_cast<const uint16_t *>(from));
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+        }
+    }
+}
+template <class T, int ROWS, int DP, int STRIDE>
+__device__ __forceinline__ void load_rows(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int bytes,
+                                          int tid, int threads) {
+    if (bytes == 16)
+        load_rows_w<T, ROWS, DP, STRIDE, 16>(dst, src, row_stride, rows, d, tid, threads);
+    else if (sizeof(T) == 4 || bytes == 4)
+        load_rows_w<T, ROWS, DP, STRIDE, 4>(dst, src, row_stride, rows, d, tid, threads);
+    else if constexpr (sizeof(T) == 2)
+        load_rows_w<T, ROWS, DP, STRIDE, 2>(dst, src, row_stride, rows, d, tid, threads);
+}
+
+// Row strides of the shared tiles, padded so that a fragment's 32 accesses
+// fall into 32 banks.
+template <class T, int DP>
+struct TileOf {
+    static constexpr int STRIDE = sizeof(T) == 4 ? DP + 4 : DP + 8;
+};
+
+// One warp's 16 query rows against tiles of keys. Scores and output use the
+// matrix instruction's layout: this lane holds rows g and g + 8 (g = lane /
+// 4) and columns 2t, 2t + 1 of each 8 (t = lane % 4).
+//
+// f16 and bf16: m16n8k16 with f32 accumulation; the probabilities are
+// rounded to the type for the second product (2^-9 or 2^-12 of each, the
+// size of the output's own rounding), the sum l keeps them unrounded.
+// f32: each product as three tf32 ones (hi*hi + hi*lo + lo*hi).
+template <class T, int DP>
+struct WarpAttn {
+    static constexpr int STRIDE = TileOf<T, DP>::STRIDE;
+    static constexpr int ND = DP / 8;
+    float o[ND][4];
+    float m[2], l[2];
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < ND; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
+    }
+
+    // s[nt] = q (16 rows from qs) . the 8 * NT keys at ks
+    template <int NT>
+    __device__ __forceinline__ void scores(float (*s)[4], uint32_t qs, uint32_t ks, int lane) const {
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t qa = qs + uint32_t(((lane & 15) * STRIDE + (lane >> 4) * 8) * 2);
+            const uint32_t ka = ks + uint32_t((((lane & 7) + (lane >> 4) * 8) * STRIDE + ((lane >> 3) & 1) * 8) * 2);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk++) {
+                uint32_t qf[4];
+                ldmatrix4(qf, qa + kk * 32);
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t kf[4];
+                    ldmatrix4(kf, ka + uint32_t(n * 8 * STRIDE * 2) + kk * 32);
+                    mma16<T>(s[n], qf, kf[0], kf[1]);
+                    mma16<T>(s[n + 1], qf, kf[2], kf[3]);
+                }
+            }
+        } else {
+            const int g = lane >> 2, t = lane & 3;
+            const uint32_t qa = qs + uint32_t((g * STRIDE + t) * 4), ka = ks + uint32_t((g * STRIDE + t) * 4);
+            // unrolled by two only: the f32 form is bound by its own matrix
+            // instructions, and more would spill
+#pragma unroll 2
+            for (int kk = 0; kk < DP / 8; kk++) {
+                uint32_t qh[4], ql[4];
+                split_tf32(lds(qa + kk * 32), qh[0], ql[0]);
+                split_tf32(lds(qa + kk * 32 + 8 * STRIDE * 4), qh[1], ql[1]);
+                split_tf32(lds(qa + kk * 32 + 16), qh[2], ql[2]);
+                split_tf32(lds(qa + kk * 32 + 8 * STRIDE * 4 + 16), qh[3], ql[3]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t h0, h1, l0, l1;
+                    split_tf32(lds(ka + uint32_t(n * 8 * STRIDE * 4) + kk * 32), h0, l0);
+                    split_tf32(lds(ka + uint32_t(n * 8 * STRIDE * 4) + kk * 32 + 16), h1, l1);
+                    mma8_tf32(s[n], ql, h0, h1);
+                    mma8_tf32(s[n], qh, l0, l1);
+                    mma8_tf32(s[n], qh, h0, h1);
+                }
+            }
+        }
+    }
+
+    static __device__ __forceinline__ float lds(uint32_t a) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+        return v;
+    }
+
+    // The softmax step over 8 * NT scores (masked ones are -inf): p in place.
+    template <int NT>
+    __device__ __forceinline__ void soften(float (*s)[4], float scale_log2) {
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
+            top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
+        }
+        float from[2], keep[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            const float now = fmaxf(m[r], top[r] * scale_log2);
+            from[r] = now == -INFINITY ? 0.0f : now;  // no key seen yet: every p is 2^-inf
+            keep[r] = exp2_fast(m[r] - from[r]);
+            m[r] = now;
+        }
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[n][e] = exp2_fast(fmaf(s[n][e], scale_log2, -from[e >> 1]));
+                sum[e >> 1] += s[n][e];
+            }
+        l[0] = fmaf(l[0], keep[0], sum[0]);
+        l[1] = fmaf(l[1], keep[1], sum[1]);
+        if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < ND; n++) {
+                o[n][0] *= keep[0];
+                o[n][1] *= keep[0];
+                o[n][2] *= keep[1];
+                o[n][3] *= keep[1];
+            }
+        }
+    }
+
+    // o += p . the 8 * NT rows at vs
+    template <int NT>
+    __device__ __forceinline__ void gather(float (*s)[4], uint32_t vs, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t va = vs + uint32_t((((lane & 7) + ((lane >> 3) & 1) * 8) * STRIDE + (lane >> 4) * 8) * 2);
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                const uint32_t pf[4] = {pack2<T>(s[n][0], s[n][1]), pack2<T>(s[n][2], s[n][3]),
+                                        pack2<T>(s[n + 1][0], s[n + 1][1]), pack2<T>(s[n + 1][2], s[n + 1][3])};
+#pragma unroll
+                for (int c = 0; c < ND; c += 2) {
+                    uint32_t vf[4];
+                    ldmatrix4_t(vf, va + uint32_t((n * 8 * STRIDE + c * 8) * 2));
+                    mma16<T>(o[c], pf, vf[0], vf[1]);
+                    mma16<T>(o[c + 1], pf, vf[2], vf[3]);
+                }
+            }
+        } else {
+            // key slots t and t + 4 of the instruction stand for keys 2t and
+            // 2t + 1, where this lane's probabilities are
+            const int g = lane >> 2, t = lane & 3;
+            const uint32_t va = vs + uint32_t((2 * t * STRIDE + g) * 4);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                uint32_t ph[4], pl[4];
+                split_tf32(s[n][0], ph[0], pl[0]);
+                split_tf32(s[n][2], ph[1], pl[1]);
+                split_tf32(s[n][1], ph[2], pl[2]);
+                split_tf32(s[n][3], ph[3], pl[3]);
+#pragma unroll
+                for (int c = 0; c < ND; c++) {
+                    uint32_t h0, h1, l0, l1;
+                    split_tf32(lds(va + uint32_t((n * 8 * STRIDE + c * 8) * 4)), h0, l0);
+                    split_tf32(lds(va + uint32_t(((n * 8 + 1) * STRIDE + c * 8) * 4)), h1, l1);
+                    mma8_tf32(o[c], pl, h0, h1);
+                    mma8_tf32(o[c], ph, l0, l1);
+                    mma8_tf32(o[c], ph, h0, h1);
+                }
+            }
+        }
+    }
+};
+
+// One output row the plain way, by a whole warp, in f32 and over the keys it
+// sees alone: for rows that came out infinite or NaN above, since there a
+// masked key's zero weight times an infinity or NaN in its values is NaN.
+template <class T>
+__device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i, int h) {
+    const int lane = threadIdx.x & 31, p = i + ln.nk - ln.nq, kvh = h / a.share;
+    const T *q = static_cast<const T *>(a.q) + (ln.q0 + i) * a.q_row + h * a.q_head;
+    const T *k = static_cast<const T *>(a.k) + ln.k0 * a.k_row + kvh * a.k_head;
+    const T *v = static_cast<const T *>(a.v) + ln.k0 * a.v_row + kvh * a.v_head;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = -INFINITY, sum = 0.0f;
+    for (int pass = 0; pass < 2; pass++) {
+        const float from = top == -INFINITY ? 0.0f : top;
+        for (int j = 0; j < ln.nk; j++) {
+            if (!sees(a, p, j)) {
+                // behind the sinks: on to the window; past it: done
+                if (a.right >= 0 && j > p + a.right) break;
+                j = max(j, p - a.left - 1);
+                continue;
+            }
+            float s = 0.0f;
+            for (int c = lane; c < a.d; c += 32) s = fmaf(to_f32(q[c]), to_f32(k[j * a.k_row + c]), s);
+#pragma unroll
+            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            s *= a.scale_log2;
+            if (pass == 0) {
+                top = (s != s || top != top) ? NAN : fmaxf(top, s);
+            } else {
+                const float w = exp2_fast(s - from);
+                sum += w;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (lane + 32 * e < a.d) acc[e] = fmaf(w, to_f32(v[j * a.v_row + lane + 32 * e]), acc[e]);
+            }
+        }
+    }
+    T *out = static_cast<T *>(a.out) + (ln.q0 + i) * a.out_row + h * a.out_head;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (lane + 32 * e < a.d) out[lane + 32 * e] = from_f32<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+}
+
+}  // namespace
+
+// Each returns a CUDA error; the grid covers any lane lengths, the hints
+// only size it.
+cudaError_t launch_attn_rows(const AttnArgs &a, int type, uint32_t max_q, cudaStream_t stream);
+cudaError_t launch_attn_split(const AttnArgs &a, int type, uint32_t max_q, uint32_t max_keys, cudaStream_t stream);
+
+}  // namespace ppocr

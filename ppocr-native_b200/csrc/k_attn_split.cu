@@ -1,0 +1,230 @@
+// Window attention for few queries a lane (single steps over a cache): the
+// keys are split, and joined in the same launch.
+//
+// Rows of a tile are the queries that read one key head (query i, head h of
+// its group), up to 16. A cluster of up to eight blocks takes one tile; its
+// 4 * blocks warps take the key tiles in turn, each with a ring of its own
+// filled by cp.async and a softmax state of its own (m, l, o). The states
+// meet through distributed shared memory: row r is joined by block r mod
+// cluster, with weights 2^(m_i - max m). No workspace, nothing to clear.
+// Bound by the keys' and values' bytes; a single lane by latency.
+#include "attn.cuh"
+
+namespace ppocr {
+
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3;
+
+template <class T, int DP>
+struct SplitTile {
+    static constexpr int BK = sizeof(T) == 4 ? 16 : 32;  // keys a warp takes at a time
+    static constexpr int STRIDE = TileOf<T, DP>::STRIDE;
+    static constexpr int Q_BYTES = 16 * STRIDE * int(sizeof(T)), K_BYTES = BK * STRIDE * int(sizeof(T));
+    static constexpr int RING = STAGES * 2 * K_BYTES;  // one warp's
+    // a warp's joined state reuses its ring: o[16][DP], m[16], l[16]
+    static_assert(RING >= (16 * DP + 32) * 4, "the state fits the ring");
+    static constexpr int SHARED = Q_BYTES + WARPS * RING;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float peer_load(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts(uint32_t addr, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
+    using R = SplitTile<T, DP>;
+    constexpr int BK = R::BK, STRIDE = R::STRIDE;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const uint32_t qs = shared_u32(smem), rings = qs + R::Q_BYTES, ring = rings + warp * R::RING;
+    const int blocks = int(cluster_size()), rank = int(cluster_rank()), workers = blocks * WARPS;
+    const Lane ln = read_lane(a, blockIdx.z);
+    const int kvh = blockIdx.y;
+    const T *k = static_cast<const T *>(a.k) + ln.k0 * a.k_row + kvh * a.k_head;
+    const T *v = static_cast<const T *>(a.v) + ln.k0 * a.v_row + kvh * a.v_head;
+    const int64_t total = int64_t(ln.nq) * a.share;
+
+    for (int64_t base = int64_t(blockIdx.x) / blocks * 16; base < total; base += int64_t(gridDim.x) / blocks * 16) {
+        const int rows = int(total - base < 16 ? total - base : 16);
+        const int shift = ln.nk - ln.nq;
+        const int p0 = int(base / a.share) + shift, p1 = int((base + rows - 1) / a.share) + shift;
+        const int pr[2] = {int((base + (lane >> 2)) / a.share) + shift, int((base + (lane >> 2) + 8) / a.share) + shift};
+        KeyTiles kt;
+        kt.plan<BK>(a, p0, p1, ln.nk);
+        const auto fetch = [&](int it, int slot) {
+            if (it < kt.n) {
+                const int j = kt.first<BK>(it), n = min(BK, kt.end(it) - j);
+                const uint32_t to = ring + uint32_t(slot * 2 * R::K_BYTES);
+                load_rows<T, BK, DP, STRIDE>(to, k + j * a.k_row, a.k_row, n, a.d, a.k_bytes, lane, 32);
+                load_rows<T, BK, DP, STRIDE>(to + R::K_BYTES, v + j * a.v_row, a.v_row, n, a.d, a.v_bytes, lane, 32);
+            }
+            copy_commit();
+        };
+        for (int r = warp; r < 16; r += WARPS) {
+            const int64_t i = (base + r) / a.share, h = kvh * a.share + (base + r) % a.share;
+            const T *src = static_cast<const T *>(a.q) + (r < rows ? (ln.q0 + i) * a.q_row + h * a.q_head : 0);
+            load_rows<T, 1, DP, STRIDE>(qs + uint32_t(r * STRIDE * int(sizeof(T))), src, 0, r < rows ? 1 : 0, a.d,
+                                        a.q_bytes, lane, 32);
+        }
+        copy_commit();
+        const int first = rank * WARPS + warp;
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; s++) fetch(first + s * workers, s);
+        copy_wait<STAGES - 1>();
+        __syncthreads();  // every warp's rows of q are there
+
+        WarpAttn<T, DP> w;
+        w.clear();
+        int slot = 0;
+        for (int it = first; it < kt.n; it += workers) {
+            copy_wait<STAGES - 2>();
+            __syncwarp();
+            fetch(it + (STAGES - 1) * workers, slot == 0 ? STAGES - 1 : slot - 1);
+            const uint32_t ks = ring + uint32_t(slot * 2 * R::K_BYTES), vs = ks + R::K_BYTES;
+            const int j0 = kt.first<BK>(it), jend = kt.end(it);
+            float s[BK / 8][4];
+            w.template scores<BK / 8>(s, qs, ks, lane);
+            const bool whole = j0 + BK <= jend && (a.right < 0 || j0 + BK - 1 <= p0 + a.right) &&
+                               (a.left < 0 || j0 >= p1 - a.left || j0 + BK <= a.sinks);
+            if (!whole) {
+#pragma unroll
+                for (int n = 0; n < BK / 8; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int j = j0 + n * 8 + (lane & 3) * 2 + (e & 1);
+                        if (j >= jend || !sees(a, pr[e >> 1], j)) s[n][e] = -INFINITY;
+                    }
+            }
+            w.template soften<BK / 8>(s, a.scale_log2);
+            w.template gather<BK / 8>(s, vs, lane);
+            slot = slot == STAGES - 1 ? 0 : slot + 1;
+        }
+        copy_wait<0>();
+        __syncwarp();  // the ring is free: this warp's state goes there
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 1);
+            w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 2);
+            const int row = (lane >> 2) + 8 * r;
+            if ((lane & 3) == 0) {
+                sts(ring + uint32_t((16 * DP + row) * 4), w.m[r]);
+                sts(ring + uint32_t((16 * DP + 16 + row) * 4), w.l[r]);
+            }
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) {
+                sts(ring + uint32_t((row * DP + n * 8 + (lane & 3) * 2) * 4), w.o[n][2 * r]);
+                sts(ring + uint32_t((row * DP + n * 8 + (lane & 3) * 2 + 1) * 4), w.o[n][2 * r + 1]);
+            }
+        }
+        cluster_sync();
+
+        for (int r = rank + warp * blocks; r < rows; r += workers) {
+            // lane x holds worker x's maximum and sum (at most 32 workers)
+            float m = -INFINITY, l = 0.0f;
+            if (lane < workers) {
+                const uint32_t at = peer_addr(rings + uint32_t((lane % WARPS) * R::RING), uint32_t(lane / WARPS));
+                m = peer_load(at + uint32_t((16 * DP + r) * 4));
+                l = peer_load(at + uint32_t((16 * DP + 16 + r) * 4));
+            }
+            float top = m;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float share = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+            float sum = l * share;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            float acc[(DP + 31) / 32] = {};
+#pragma unroll 4
+            for (int x = 0; x < workers; x++) {
+                const float c = __shfl_sync(0xffffffffu, share, x);
+                const uint32_t at = peer_addr(rings + uint32_t((x % WARPS) * R::RING), uint32_t(x / WARPS));
+#pragma unroll
+                for (int e = 0; e < (DP + 31) / 32; e++)
+                    if (lane + 32 * e < DP) acc[e] = fmaf(c, peer_load(at + uint32_t((r * DP + lane + 32 * e) * 4)), acc[e]);
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < (DP + 31) / 32; e++) {
+                acc[e] *= inv;
+                bad |= !(fabsf(acc[e]) < INFINITY);
+            }
+            const int i = int((base + r) / a.share), h = kvh * a.share + int((base + r) % a.share);
+            if (__any_sync(0xffffffffu, bad)) {
+                row_alone<T>(a, ln, i, h);
+            } else {
+                T *out = static_cast<T *>(a.out) + (ln.q0 + i) * a.out_row + h * a.out_head;
+#pragma unroll
+                for (int e = 0; e < (DP + 31) / 32; e++)
+                    if (lane + 32 * e < a.d) out[lane + 32 * e] = from_f32<T>(acc[e]);
+            }
+        }
+        cluster_sync();  // no block overwrites or leaves what another still reads
+    }
+}
+
+template <class T, int DP>
+cudaError_t start_split(const AttnArgs &a, uint32_t max_q, uint32_t max_keys, cudaStream_t stream) {
+    using R = SplitTile<T, DP>;
+    cudaError_t e = raise_shared<attn_split_kernel<T, DP>>(R::SHARED);
+    if (e != cudaSuccess) return e;
+    const uint64_t rows = uint64_t(max_q) * a.share, tiles = rows ? (rows + 15) / 16 : 1;
+    const uint64_t alone = tiles * a.lanes * a.kv_heads;
+    // blocks a tile: until the card is full or every warp has one key tile
+    uint32_t blocks = 1;
+    while (blocks < 8 && alone * blocks < uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(unsigned(tiles * blocks), unsigned(a.kv_heads), unsigned(a.lanes));
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = R::SHARED;
+    c.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = blocks;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, attn_split_kernel<T, DP>, a);
+}
+
+template <class T>
+cudaError_t start_split_d(const AttnArgs &a, uint32_t max_q, uint32_t max_keys, cudaStream_t stream) {
+    if (a.d <= 16) return start_split<T, 16>(a, max_q, max_keys, stream);
+    if (a.d <= 32) return start_split<T, 32>(a, max_q, max_keys, stream);
+    if (a.d <= 64) return start_split<T, 64>(a, max_q, max_keys, stream);
+    return start_split<T, 128>(a, max_q, max_keys, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_split(const AttnArgs &a, int type, uint32_t max_q, uint32_t max_keys, cudaStream_t stream) {
+    if (type == PPOCR_F32) return start_split_d<float>(a, max_q, max_keys, stream);
+    if (type == PPOCR_F16) return start_split_d<__half>(a, max_q, max_keys, stream);
+    return start_split_d<__nv_bfloat16>(a, max_q, max_keys, stream);
+}
+
+}  // namespace ppocr

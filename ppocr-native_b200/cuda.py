@@ -65,6 +65,10 @@ _SIG = {
                                            ctypes.c_size_t, ctypes.POINTER(ctypes.c_double),
                                            ctypes.POINTER(ctypes.c_double), ctypes.c_void_p, ctypes.c_size_t,
                                            ctypes.c_void_p]),
+    # transformer-block operators
+    "ppocr_attention_window": (ctypes.c_int, [ctypes.c_void_p] * 9),
+    "ppocr_rms_norm_e4m3": (ctypes.c_int, [ctypes.c_void_p] * 8),
+    "ppocr_matvec_q4": (ctypes.c_int, [ctypes.c_void_p] * 9),
     # page steps and the reader
     "ppocr_reader_options_default": (None, [ctypes.c_void_p]),
     "ppocr_reader_create": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t,
@@ -337,6 +341,98 @@ def db_mask(prob: int, pixels: int, thresh: float, mask: int, stream: int | None
     """The DB text mask prob > thresh (device pointers as ints); see
     `ppocr_db_mask` in include/ppocr_cuda.h."""
     _check(lib().ppocr_db_mask(prob, pixels, thresh, mask, stream or None))
+
+
+# ------------------------------------------- transformer-block operators
+
+TYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}
+
+
+class AttentionShape(ctypes.Structure):
+    """`ppocr_attention_shape`: a layer's sizes, kept by the caller across
+    calls. Types by name ("f32", "f16", "bf16"); strides as (row, head) pairs
+    in elements, None for rows of `heads` x `head_dim` elements side by side;
+    left, right -1 for no limit."""
+
+    _fields_ = [("type", ctypes.c_int32), ("lanes", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("left", ctypes.c_int32),
+                ("right", ctypes.c_int32), ("sinks", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("max_q", ctypes.c_uint32), ("max_k", ctypes.c_uint32), ("q_rows", ctypes.c_uint64),
+                ("kv_rows", ctypes.c_uint64), ("q_row", ctypes.c_uint64), ("q_head", ctypes.c_uint64),
+                ("k_row", ctypes.c_uint64), ("k_head", ctypes.c_uint64), ("v_row", ctypes.c_uint64),
+                ("v_head", ctypes.c_uint64), ("out_row", ctypes.c_uint64), ("out_head", ctypes.c_uint64)]
+
+    def __init__(self, type: str, lanes: int, heads: int, kv_heads: int, head_dim: int, q_rows: int, kv_rows: int,
+                 scale: float, left: int = -1, right: int = -1, sinks: int = 0, q_strides=None, k_strides=None,
+                 v_strides=None, out_strides=None, max_q: int = 0, max_k: int = 0):
+        rows = (heads * head_dim, head_dim), (kv_heads * head_dim, head_dim)
+        q, k, v, out = q_strides or rows[0], k_strides or rows[1], v_strides or rows[1], out_strides or rows[0]
+        super().__init__(_type(type), lanes, heads, kv_heads, head_dim, left, right, sinks, scale, max_q, max_k,
+                         q_rows, kv_rows, *q, *k, *v, *out)
+        self.ref = ctypes.addressof(self)
+
+
+class RmsNormShape(ctypes.Structure):
+    """`ppocr_rms_norm_shape`; strides in elements, 0 for rows side by side."""
+
+    _fields_ = [("type", ctypes.c_int32), ("channels", ctypes.c_uint32), ("group", ctypes.c_uint32),
+                ("eps", ctypes.c_float), ("rows", ctypes.c_uint64), ("x_row", ctypes.c_uint64),
+                ("residual_row", ctypes.c_uint64), ("sum_row", ctypes.c_uint64), ("y_row", ctypes.c_uint64)]
+
+    def __init__(self, type: str, rows: int, channels: int, group: int = 0, eps: float = 1e-6, x_row: int = 0,
+                 residual_row: int = 0, sum_row: int = 0, y_row: int = 0):
+        super().__init__(_type(type), channels, group, eps, rows, x_row, residual_row, sum_row, y_row)
+        self.ref = ctypes.addressof(self)
+
+
+class MatvecQ4Shape(ctypes.Structure):
+    """`ppocr_matvec_q4_shape`; x_row and y_row in elements, w_row in bytes, 0
+    for rows side by side."""
+
+    _fields_ = [("x_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("scale_type", ctypes.c_int32),
+                ("rows", ctypes.c_uint32), ("k", ctypes.c_uint32), ("n", ctypes.c_uint32), ("group", ctypes.c_uint32),
+                ("x_group", ctypes.c_uint32), ("x_row", ctypes.c_uint64), ("y_row", ctypes.c_uint64),
+                ("w_row", ctypes.c_uint64)]
+
+    def __init__(self, x_type: str, y_type: str, scale_type: str, rows: int, k: int, n: int, group: int,
+                 x_group: int = 0, x_row: int = 0, y_row: int = 0, w_row: int = 0):
+        super().__init__(_type(x_type), _type(y_type), _type(scale_type), rows, k, n, group, x_group, x_row, y_row,
+                         w_row)
+        self.ref = ctypes.addressof(self)
+
+
+def _type(name: str) -> int:
+    if name not in TYPES:
+        raise ValueError(f"unknown element type {name!r}: one of {', '.join(TYPES)}")
+    return TYPES[name]
+
+
+def attention_window(shape: AttentionShape, q: int, k: int, v: int, out: int, q_offsets: int,
+                     k_begin: int | None = None, k_len: int | None = None, stream: int | None = None) -> None:
+    """Attention with a sliding window and sinks over packed lanes (device
+    pointers as ints); see `ppocr_attention_window` in include/ppocr_cuda.h."""
+    code = lib().ppocr_attention_window(shape.ref, q, k, v, out, q_offsets, k_begin, k_len, stream)
+    if code:
+        _check(code)
+
+
+def rms_norm_e4m3(shape: RmsNormShape, x: int, residual: int | None, gamma: int, sum: int | None, y: int, scales: int,
+                  stream: int | None = None) -> None:
+    """The residual's addition, a root-mean-square norm and its 8-bit output
+    (device pointers as ints); see `ppocr_rms_norm_e4m3` in
+    include/ppocr_cuda.h."""
+    code = lib().ppocr_rms_norm_e4m3(shape.ref, x, residual, gamma, sum, y, scales, stream)
+    if code:
+        _check(code)
+
+
+def matvec_q4(shape: MatvecQ4Shape, x: int, x_scales: int | None, w: int, scales: int, zeros: int | None,
+              bias: int | None, y: int, stream: int | None = None) -> None:
+    """A few rows of x times 4-bit weights (device pointers as ints); see
+    `ppocr_matvec_q4` in include/ppocr_cuda.h."""
+    code = lib().ppocr_matvec_q4(shape.ref, x, x_scales, w, scales, zeros, bias, y, stream)
+    if code:
+        _check(code)
 
 
 # ---------------------------------------------------------------- page steps
