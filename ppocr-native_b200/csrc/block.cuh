@@ -3,6 +3,7 @@
 // instructions, asynchronous copies, and the checks of their C entry points.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -12,6 +13,7 @@
 #include <string>
 
 #include "../../include/ppocr_cuda.h"
+#include "async.cuh"
 
 namespace ppocr {
 
@@ -73,6 +75,23 @@ cudaError_t raise_shared(int bytes) {
     return e;
 }
 
+// The driver's tensor-map encoder (NULL where it has none).
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled tensor_map_encoder() {
+    static const EncodeTiled fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
 inline size_t type_size(int type) { return type == PPOCR_F32 ? 4 : type == PPOCR_E4M3 ? 1 : 2; }
 
 // True when the byte ranges [a, a + an) and [b, b + bn) meet.
@@ -132,6 +151,16 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A wait on an mbarrier's phase that ends by itself: a copy takes
+// microseconds, and after two seconds the caller is told so (false).
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity) {
+    if (try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    while (!try_wait_sleep(bar, parity, 20000u))
+        if (global_ns() - t0 > 2000000000ull) return false;
+    return true;
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t r[4], uint32_t addr) {

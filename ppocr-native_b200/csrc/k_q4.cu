@@ -12,11 +12,13 @@
 // both operands agree, so a lane's four k slots of two instructions are 8
 // consecutive weights, one 32-bit word, and x is staged in that order.
 //
-// A block of 8 warps takes 8 / WK row tiles at a time, WK warps a tile, each
-// every WK-th step of 128 k; weights come through a ring of cp.async stages
-// per warp that runs on across tiles, x lies in shared memory (in chunks of
-// k where it does not fit), and the WK partial sums meet there in a fixed
-// order. Bound by the weights' bytes.
+// A block of 8 warps takes 8 / wk row tiles at a time, wk warps a tile, each
+// every wk-th step of k; weights come through a ring of cp.async stages per
+// warp that runs on across tiles, x lies in shared memory, and the wk partial
+// sums meet there in a fixed order. Where x is too much for one block, or the
+// tiles are too few for the card, a cluster's blocks share k and their sums
+// meet through distributed shared memory (past eight blocks' worth of x, it
+// is staged in chunks). Bound by the weights' bytes.
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -28,14 +30,6 @@ namespace ppocr {
 namespace {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int STEP = 128;               // k a warp takes at a time: 64 bytes of each of 16 rows
-constexpr int STAGES = 4;
-constexpr int W_BYTES = 16 * 64;        // a stage's weights
-constexpr int S_BYTES = 16 * 4 * 8;     // a stage's (scale, zero point) per row and 32 k
-constexpr int RING = STAGES * (W_BYTES + S_BYTES);
-// Staged x: two blocks an SM with up to 16 columns, one with 32 (whose 8 warps'
-// turn of x takes 64 KB).
-constexpr int x_bytes_of(int ct) { return (ct <= 2 ? 40 : 64) * 1024; }
 
 struct Q4Args {
     const void *x;
@@ -49,8 +43,10 @@ struct Q4Args {
     int m, k, n, group, groups;
     int scale_type, y_type;
     int x_groups;   // scales a row of x has (e4m3): 0 none, 1 the row's, else one a group
-    int wk;         // warps that share a row tile
-    int steps, chunk_steps, cols_rows;  // steps of k in all and per staged chunk; rows of x a pass takes
+    int cols_rows;  // rows of x a pass takes
+    int ks, wk;     // blocks of a cluster, and warps of a block, that share a row tile
+    int steps, share_steps, chunk_steps;  // of k: in all, a block's share, staged at a time
+    int keep;       // lists of tiles whose partial sums a cluster gathers before it joins them
     bool w_vec, x_vec;
 };
 
@@ -173,89 +169,156 @@ __device__ __forceinline__ float part_of(float x, int part) {
     return part == 0 ? hi : part == 1 ? mid : rest - mid;
 }
 
-// BPG: 32-k blocks a weight group, 1, 2 or 4 (1 serves every multiple of 32).
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_load(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+
+// A step: 256 k, 128 bytes of each of a tile's 16 rows of weights, swizzled as
+// the tensor copies do (16-byte chunk c of row r at c ^ (r % 8)).
+constexpr int STEP = 256, BLOCKS = STEP / 32, ROW = STEP / 2, W_BYTES = 16 * ROW;
+
+// Sizes of one variant. CT: 8-column tiles of x; BPG: 32-k blocks a weight
+// group (4, 2, or 1, which serves every multiple of 32).
+template <int CT, int BPG, bool ZEROS>
+struct Q4Tile {
+    static constexpr int COLS = 8 * CT;
+    static constexpr int SB = BLOCKS / BPG;  // scales a row and step
+    static constexpr int SPL = SB / 2;       // of which a lane fetches
+    static constexpr int S_BYTES = 16 * SB * (ZEROS ? 8 : 4);
+    static constexpr int STAGES = CT <= 2 ? 3 : 4;
+    // weights of every warp and stage first (the swizzle wants 1 KB borders),
+    // then the scales, the partial sums, the barriers, 64 zeros and x
+    static constexpr int SCALES = WARPS * STAGES * W_BYTES, RED = SCALES + WARPS * STAGES * S_BYTES;
+    static constexpr int BARS = RED + 2 * WARPS * 16 * COLS * 4, ZERO = BARS + WARPS * STAGES * 8, FIXED = ZERO + 64;
+    // staged x and, behind it, a cluster's partial results (one list at least);
+    // two blocks an SM up to 16 columns
+    static constexpr int X_BYTES = (CT == 1 ? 24 : CT == 2 ? 16 : 64) * 1024, PART_BYTES = (CT == 4 ? 16 : 8) * 1024;
+    static_assert(CT > 2 || FIXED + X_BYTES + PART_BYTES <= 113 * 1024, "two blocks an SM");
+    static_assert(PART_BYTES >= WARPS * 16 * COLS * 4, "one list of partial results");
+};
+
 template <class XT, int CT, int BPG, bool ZEROS>
-__global__ void __launch_bounds__(THREADS, CT <= 2 ? 2 : 1) q4_kernel(const __grid_constant__ Q4Args a) {
+__global__ void __launch_bounds__(THREADS, CT <= 2 ? 2 : 1)
+    q4_kernel(const __grid_constant__ Q4Args a, const __grid_constant__ CUtensorMap map) {
     using M = typename Enter<XT>::M;
-    constexpr int PARTS = Enter<XT>::PARTS, COLS = 8 * CT;
-    extern __shared__ __align__(16) unsigned char smem[];
+    using Q = Q4Tile<CT, BPG, ZEROS>;
+    constexpr int PARTS = Enter<XT>::PARTS, COLS = Q::COLS, STAGES = Q::STAGES, SB = Q::SB;
+    extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    unsigned char *ring = smem + warp * RING;
-    float *red = reinterpret_cast<float *>(smem + WARPS * RING);          // [2][WARPS][16][COLS]
-    unsigned char *xs = smem + WARPS * RING + 2 * WARPS * 16 * COLS * 4;  // [block][cols][t] of 16 bytes
-    const uint32_t ring_s = shared_u32(ring), xs_s = shared_u32(xs);
+    unsigned char *ring = smem + warp * STAGES * W_BYTES, *sring = smem + Q::SCALES + warp * STAGES * Q::S_BYTES;
+    float *red = reinterpret_cast<float *>(smem + Q::RED);  // [2][WARPS][16][COLS]
+    unsigned char *xs = smem + Q::FIXED;                    // [block][column][t] of 16 bytes
+    const uint32_t ring_s = shared_u32(ring), bars = shared_u32(smem + Q::BARS) + warp * STAGES * 8;
 
+    // this block's share of k (one of a cluster's blocks) and of the tiles
+    const int ks = a.ks, rank = ks > 1 ? int(blockIdx.x) % ks : 0, team = int(blockIdx.x) / ks, teams = int(gridDim.x) / ks;
+    const int s_lo = rank * a.share_steps, s_hi = min(a.steps, s_lo + a.share_steps);
     const int wr = WARPS / a.wk, k_warp = warp % a.wk, r_warp = warp / a.wk;
-    const int tiles = (a.n + 15) / 16, turns = (a.steps + a.wk - 1) / a.wk;
-    const int m0 = blockIdx.y * a.cols_rows, rows = min(a.cols_rows, a.m - m0), cols = rows * PARTS;
-    const bool once = a.chunk_steps >= a.steps;
+    const int tiles = (a.n + 15) / 16, turns = (a.share_steps + a.wk - 1) / a.wk;
+    const int m0 = blockIdx.y * a.cols_rows, rows = min(a.cols_rows, a.m - m0);
+    // x's columns: as many as there are for one column tile, else whole tiles
+    const int cols = CT == 1 ? rows * PARTS : COLS;
+    const bool once = a.chunk_steps >= a.share_steps;
+    const int lists = (tiles + wr - 1) / wr, my_lists = lists > team ? (lists - team + teams - 1) / teams : 0;
+    float *part = reinterpret_cast<float *>(xs + a.chunk_steps * BLOCKS * 64 * cols);
 
-    // x's chunk from step `s0` on into shared memory
+    if (lane == 0)
+        for (int s = 0; s < STAGES; s++) bar_init(bars + s * 8, 1);
+    if (tid < 16) reinterpret_cast<uint32_t *>(smem + Q::ZERO)[tid] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+
+    // x's chunk of steps from `s0` on into shared memory. Groups of 128 k: a
+    // lane's four words of a row are 32 consecutive weights, so k is staged in
+    // that order (one 16-byte load a row); else a lane's word is its 8 k of a block.
     const auto stage_x = [&](int s0) {
-        const int blocks = min(a.chunk_steps, a.steps - s0) * 4;
-        for (int e = tid; e < blocks * rows * 4; e += THREADS) {
-            const int q = e & 3, r = (e >> 2) % rows, b = (e >> 2) / rows;
-            float v[8];
-            load_x<XT>(a, m0 + r, (s0 * 4 + b) * 32 + q * 8, v);
+        const int blocks = max(0, min(a.chunk_steps, s_hi - s0)) * BLOCKS, q = tid & 3;
+        for (int b = tid >> 2; b < blocks; b += THREADS / 4) {
+            const int k = s0 * STEP + (BPG == 4 ? (b >> 2) * 128 + q * 32 + (b & 3) * 8 : b * 32 + q * 8);
+            for (int r = 0; r < (CT == 1 ? rows : COLS / PARTS); r++) {
+                float v[8] = {};
+                if (r < rows) load_x<XT>(a, m0 + r, k, v);
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) {
-                uint32_t u[4];
+                for (int p = 0; p < PARTS; p++) {
+                    uint32_t u[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) u[i] = pack2<M>(part_of<XT>(v[i], part), part_of<XT>(v[i + 4], part));
-                *reinterpret_cast<uint4 *>(xs + ((b * cols + r * PARTS + part) * 4 + q) * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+                    for (int i = 0; i < 4; i++) u[i] = pack2<M>(part_of<XT>(v[i], p), part_of<XT>(v[i + 4], p));
+                    *reinterpret_cast<uint4 *>(xs + ((b * cols + r * PARTS + p) * 4 + q) * 16) = make_uint4(u[0], u[1], u[2], u[3]);
+                }
             }
+            if constexpr (CT > 1 && COLS % PARTS != 0)
+                for (int c = COLS / PARTS * PARTS; c < COLS; c++)
+                    *reinterpret_cast<uint4 *>(xs + ((b * cols + c) * 4 + q) * 16) = make_uint4(0, 0, 0, 0);
         }
     };
 
-    // this warp's u-th step: tile (u / turns) of its block's list, turn u % turns
-    const int first_tile = blockIdx.x * wr + r_warp, tile_step = gridDim.x * wr;
-    const int groups_of_tiles = (tiles + wr - 1) / wr;
-    const int my_groups = groups_of_tiles > int(blockIdx.x) ? (groups_of_tiles - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x) : 0;
-
-    // prefetch cursor
-    int f_tile = first_tile, f_turn = 0, f_left = my_groups * turns;
-    float2 held[2] = {};  // scales and zero points on their way to shared memory
+    // the prefetch cursor: the tile it is at, this lane's scales there
+    const int s_row = lane >> 1, s_col = (lane & 1) * Q::SPL;
+    int f_tile = team * wr + r_warp, f_turn = 0, f_left = my_lists * turns;
+    float held[Q::SPL] = {};
+    uint32_t held_z[Q::SPL] = {};
     const auto fetch = [&](int slot) {
-        if (f_left > 0) {
-            const int step = f_turn * a.wk + k_warp;
-            const bool on = f_tile < tiles && step < a.steps;
-            if (on) {
-                const uint32_t to = ring_s + slot * (W_BYTES + S_BYTES);
-                const int half_k = (a.k + 1) / 2;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int r = (lane >> 2) + 8 * i, c = lane & 3, n = f_tile * 16 + r, at = step * 64 + c * 16;
-                    int valid = n < a.n ? half_k - at : 0;
-                    valid = valid < 0 ? 0 : valid > 16 ? 16 : valid;
-                    const uint8_t *from = valid ? a.w + int64_t(n) * a.w_row + at : a.w;
-                    const int place = r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
-                    if (a.w_vec) {
-                        copy_async<16>(to + place, from, valid);
-                    } else {
-                        for (int j = 0; j < 16; j++) ring[slot * (W_BYTES + S_BYTES) + place + j] = j < valid ? from[j] : 0;
-                    }
+        if (f_left <= 0) return;
+        const int step = s_lo + f_turn * a.wk + k_warp;
+        if (f_tile < tiles && step < s_hi) {
+            if (a.w_vec) {
+                if (lane == 0) {
+                    arrive_expect(bars + slot * 8, W_BYTES);
+                    tma_load_2d(ring_s + slot * W_BYTES, &map, step * ROW, f_tile * 16, bars + slot * 8);
                 }
-                const int n = f_tile * 16 + (lane >> 1);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int group = ((step * 4 + (lane & 1) * 2 + i) * 32) / a.group;
-                    held[i] = make_float2(0.0f, __uint_as_float(8u));
-                    if (n < a.n && group < a.groups) {
-                        const int64_t at = int64_t(n) * a.groups + group;
-                        held[i].x = load_scale(a, at) * Enter<XT>::SCALE;
-                        if constexpr (ZEROS) held[i].y = __uint_as_float(uint32_t(a.zeros[at]) & 15u);
-                    }
+            } else {
+                const int half_k = (a.k + 1) / 2, at = step * ROW;
+                for (int e = lane; e < W_BYTES; e += 32) {
+                    const int r = e / ROW, c = e % ROW, n = f_tile * 16 + r;
+                    ring[slot * W_BYTES + r * ROW + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)] =
+                        n < a.n && at + c < half_k ? a.w[int64_t(n) * a.w_row + at + c] : 0;
                 }
             }
-            f_left--;
-            if (++f_turn == turns) f_turn = 0, f_tile += tile_step;
+            const int n = f_tile * 16 + s_row;
+            const int64_t row = int64_t(n) * a.groups;
+#pragma unroll
+            for (int i = 0; i < Q::SPL; i++) {
+                const int b = step * SB + s_col + i, group = a.group == 32 * BPG ? b : b * BPG * 32 / a.group;
+                held[i] = 0.0f;
+                held_z[i] = 8;
+                if (n < a.n && group < a.groups) {
+                    held[i] = load_scale(a, row + group) * Enter<XT>::SCALE;
+                    if constexpr (ZEROS) held_z[i] = uint32_t(__ldg(a.zeros + row + group)) & 15u;
+                }
+            }
         }
-        copy_commit();
+        f_left--;
+        if (++f_turn == turns) {
+            f_turn = 0;
+            f_tile += teams * wr;
+        }
     };
     const auto put_scales = [&](int slot) {
-        float2 *s = reinterpret_cast<float2 *>(ring + slot * (W_BYTES + S_BYTES) + W_BYTES);
-        s[(lane >> 1) * 4 + (lane & 1) * 2] = held[0];
-        s[(lane >> 1) * 4 + (lane & 1) * 2 + 1] = held[1];
+        unsigned char *s = sring + slot * Q::S_BYTES;
+#pragma unroll
+        for (int i = 0; i < Q::SPL; i++) {
+            if constexpr (ZEROS)
+                reinterpret_cast<float2 *>(s)[s_row * SB + s_col + i] = make_float2(held[i], __uint_as_float(held_z[i]));
+            else
+                reinterpret_cast<float *>(s)[s_row * SB + s_col + i] = held[i];
+        }
     };
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++) {
@@ -263,123 +326,205 @@ __global__ void __launch_bounds__(THREADS, CT <= 2 ? 2 : 1) q4_kernel(const __gr
         put_scales(s);
     }
     if (once) {
-        stage_x(0);
+        stage_x(s_lo);
         __syncthreads();
     }
 
-    int slot = 0, buf = 0;
-    for (int list = 0; list < my_groups; list++) {
-        const int tile = first_tile + list * tile_step;
+    // one output value: the row's scale, the bias, the type
+    const auto finish = [&](int m, int n, float y) {
+        if (sizeof(XT) == 1 && a.x_groups == 1) y *= __ldg(a.x_scales + m0 + m);
+        if (a.bias) y += __ldg(a.bias + n);
+        const int64_t at = int64_t(m0 + m) * a.y_row + n;
+        if (a.y_type == PPOCR_F32)
+            static_cast<float *>(a.y)[at] = y;
+        else if (a.y_type == PPOCR_F16)
+            static_cast<__half *>(a.y)[at] = __float2half_rn(y);
+        else
+            static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(y);
+    };
+
+    // the instruction's rows g and g + 8 are the tile's rows `my` and my + 8: an
+    // order in which the rows that one phase of a 16-byte load reads lie in different banks
+    const int my = (g >> 1) | ((g & 1) << 2);
+    const uint32_t w_at = uint32_t(my * ROW), key = uint32_t(my) << 4;
+    // lanes with no column of x (one column tile) read zeros
+    const bool has_x = CT > 1 || g < cols;
+    const uint32_t x_at = has_x ? shared_u32(xs) + uint32_t(g * 64 + t * 16) : shared_u32(smem + Q::ZERO);
+    const uint32_t x_step = has_x ? uint32_t(cols * 64) : 0;
+    int slot = 0, buf = 0, kept = 0;
+    uint32_t phase = 0;  // bit s: the parity stage s's next copy completes
+    bool late = false;   // a copy that never came: the results say so
+    for (int list = 0; list < my_lists; list++) {
+        const int tile = (team + list * teams) * wr + r_warp;
         float acc[CT][4] = {};
         for (int turn = 0; turn < turns; turn++) {
-            const int step = turn * a.wk + k_warp;
+            const int step = s_lo + turn * a.wk + k_warp;
             if (!once && (turn * a.wk) % a.chunk_steps == 0) {
                 __syncthreads();
-                stage_x(turn * a.wk);
+                stage_x(s_lo + turn * a.wk);
                 __syncthreads();
             }
-            copy_wait<STAGES - 2>();
-            __syncwarp();
+            const bool on = tile < tiles && step < s_hi;
+            __syncwarp();  // the stage before is read, its scales' successors written
             const int next = slot == 0 ? STAGES - 1 : slot - 1;
             fetch(next);
-            if (tile < tiles && step < a.steps) {
-                const unsigned char *ws = ring + slot * (W_BYTES + S_BYTES);
-                const float2 *ss = reinterpret_cast<const float2 *>(ws + W_BYTES);
-                const int b0 = (once ? step : step % a.chunk_steps) * 4;
+            if (on) {
+                if (a.w_vec) {
+                    if (!late && !wait_copy(bars + slot * 8, (phase >> slot) & 1u)) late = true;
+                    phase ^= 1u << slot;
+                }
+                const uint32_t ws = ring_s + uint32_t(slot * W_BYTES) + w_at;
+                const unsigned char *ss = sring + slot * Q::S_BYTES;
+                int in = step - s_lo;
+                if (!once) in %= a.chunk_steps;
+                uint32_t xb = x_at + uint32_t(in * BLOCKS) * x_step;
+                const int blocks = min(BLOCKS, (a.k - step * STEP + 31) / 32);
 #pragma unroll
-                for (int b = 0; b < 4; b += BPG) {
+                for (int b = 0; b < BLOCKS; b += BPG) {
+                    if (b > 0 && b >= blocks) break;
                     float sum[CT][4] = {};
-                    const float2 s0 = ss[g * 4 + b], s1 = ss[(g + 8) * 4 + b];
-                    const uint32_t z0 = ZEROS ? __float_as_uint(s0.y) : 8u, z1 = ZEROS ? __float_as_uint(s1.y) : 8u;
+                    float s0, s1;
+                    uint32_t z0 = 8, z1 = 8;
+                    if constexpr (ZEROS) {
+                        const float2 u0 = reinterpret_cast<const float2 *>(ss)[my * SB + b / BPG];
+                        const float2 u1 = reinterpret_cast<const float2 *>(ss)[(my + 8) * SB + b / BPG];
+                        s0 = u0.x, s1 = u1.x, z0 = __float_as_uint(u0.y), z1 = __float_as_uint(u1.y);
+                    } else {
+                        s0 = reinterpret_cast<const float *>(ss)[my * SB + b / BPG];
+                        s1 = reinterpret_cast<const float *>(ss)[(my + 8) * SB + b / BPG];
+                    }
+                    uint32_t w0[BPG], w1[BPG];
+                    if constexpr (BPG == 4) {
+                        const uint32_t at = ws + (uint32_t((b + t) << 4) ^ key);
+                        const uint4 u0 = lds128(at), u1 = lds128(at + 8 * ROW);
+                        w0[0] = u0.x, w0[1] = u0.y, w0[2] = u0.z, w0[3] = u0.w;
+                        w1[0] = u1.x, w1[1] = u1.y, w1[2] = u1.z, w1[3] = u1.w;
+                    } else {
 #pragma unroll
-                    for (int c = b; c < b + BPG; c++) {
-                        const int at = ((c ^ ((g >> 1) & 3)) * 16) + t * 4;
-                        const uint32_t w0 = *reinterpret_cast<const uint32_t *>(ws + g * 64 + at);
-                        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(ws + (g + 8) * 64 + at);
+                        for (int c = 0; c < BPG; c++) {
+                            const uint32_t at = ws + (uint32_t((b + c) << 4) ^ key) + t * 4;
+                            w0[c] = lds32(at);
+                            w1[c] = lds32(at + 8 * ROW);
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < BPG; c++) {
                         uint32_t p0[4], p1[4];
-                        unpack<M>(w0, z0, p0);
-                        unpack<M>(w1, z1, p1);
+                        unpack<M>(w0[c], z0, p0);
+                        unpack<M>(w1[c], z1, p1);
                         const uint32_t lo[4] = {p0[0], p1[0], p0[1], p1[1]}, hi[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) {
-                            const int col = ct * 8 + g;
-                            uint4 xf = make_uint4(0, 0, 0, 0);
-                            if (col < cols)
-                                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                             : "=r"(xf.x), "=r"(xf.y), "=r"(xf.z), "=r"(xf.w)
-                                             : "r"(xs_s + uint32_t((((b0 + c) * cols + col) * 4 + t) * 16)));
+                            const uint4 xf = lds128(CT == 1 ? xb : xb + uint32_t(((b + c) * COLS + ct * 8) * 64));
                             mma16<M>(sum[ct], lo, xf.x, xf.y);
                             mma16<M>(sum[ct], hi, xf.z, xf.w);
                         }
+                        if constexpr (CT == 1) xb += x_step;
                     }
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
                         float f0 = 1.0f, f1 = 1.0f;
                         if (sizeof(XT) == 1 && a.x_groups > 1) {
-                            const int group = (step * 4 + b) * 32 / a.group, c0 = ct * 8 + t * 2;
+                            const int group = (step * BLOCKS + b) * 32 / a.group, c0 = ct * 8 + t * 2;
                             if (group < a.groups) {
                                 if (c0 < rows) f0 = __ldg(a.x_scales + int64_t(m0 + c0) * a.x_groups + group);
                                 if (c0 + 1 < rows) f1 = __ldg(a.x_scales + int64_t(m0 + c0 + 1) * a.x_groups + group);
                             }
                         }
-                        acc[ct][0] = fmaf(sum[ct][0], s0.x * f0, acc[ct][0]);
-                        acc[ct][1] = fmaf(sum[ct][1], s0.x * f1, acc[ct][1]);
-                        acc[ct][2] = fmaf(sum[ct][2], s1.x * f0, acc[ct][2]);
-                        acc[ct][3] = fmaf(sum[ct][3], s1.x * f1, acc[ct][3]);
+                        acc[ct][0] = fmaf(sum[ct][0], s0 * f0, acc[ct][0]);
+                        acc[ct][1] = fmaf(sum[ct][1], s0 * f1, acc[ct][1]);
+                        acc[ct][2] = fmaf(sum[ct][2], s1 * f0, acc[ct][2]);
+                        acc[ct][3] = fmaf(sum[ct][3], s1 * f1, acc[ct][3]);
                     }
                 }
             }
             put_scales(next);
             slot = slot == STAGES - 1 ? 0 : slot + 1;
         }
+        if (late) acc[0][0] = acc[0][1] = acc[0][2] = acc[0][3] = NAN;
         // the warps' partial sums: [warp][row of the tile][column]
         float *mine = red + (buf * WARPS + warp) * 16 * COLS;
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            *reinterpret_cast<float2 *>(mine + g * COLS + ct * 8 + t * 2) = make_float2(acc[ct][0], acc[ct][1]);
-            *reinterpret_cast<float2 *>(mine + (g + 8) * COLS + ct * 8 + t * 2) = make_float2(acc[ct][2], acc[ct][3]);
+            *reinterpret_cast<float2 *>(mine + my * COLS + ct * 8 + t * 2) = make_float2(acc[ct][0], acc[ct][1]);
+            *reinterpret_cast<float2 *>(mine + (my + 8) * COLS + ct * 8 + t * 2) = make_float2(acc[ct][2], acc[ct][3]);
         }
         __syncthreads();
-        if (tile < tiles) {
-            const float *from = red + (buf * WARPS + r_warp * a.wk) * 16 * COLS;
-            for (int e = k_warp * 32 + lane; e < 16 * rows; e += a.wk * 32) {
-                const int r = e & 15, m = e >> 4, n = tile * 16 + r;
-                if (n >= a.n) continue;
-                float y = 0.0f;
-                for (int p = PARTS - 1; p >= 0; p--)
-                    for (int w = 0; w < a.wk; w++) y += from[(w * 16 + r) * COLS + m * PARTS + p];
-                if (sizeof(XT) == 1 && a.x_groups == 1) y *= __ldg(a.x_scales + m0 + m);
-                if (a.bias) y += __ldg(a.bias + n);
-                const int64_t at = int64_t(m0 + m) * a.y_row + n;
-                if (a.y_type == PPOCR_F32)
-                    static_cast<float *>(a.y)[at] = y;
-                else if (a.y_type == PPOCR_F16)
-                    static_cast<__half *>(a.y)[at] = __float2half_rn(y);
-                else
-                    static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(y);
-            }
+        const float *from = red + (buf * WARPS + r_warp * a.wk) * 16 * COLS;
+        for (int e = k_warp * 32 + lane; e < 16 * rows; e += a.wk * 32) {
+            const int r = e & 15, m = e >> 4, n = tile * 16 + r;
+            float y = 0.0f;
+            for (int p = PARTS - 1; p >= 0; p--)
+                for (int w = 0; w < a.wk; w++) y += from[(w * 16 + r) * COLS + m * PARTS + p];
+            if (ks > 1)
+                part[(kept * wr + r_warp) * 16 * rows + e] = y;
+            else if (n < a.n)
+                finish(m, n, y);
         }
         buf ^= 1;  // the next tile's sums go elsewhere: one barrier a tile
+        if (ks > 1 && (++kept == a.keep || list + 1 == my_lists)) {
+            // the cluster's sums over k, in rank order; block `rank` joins every
+            // ks-th value
+            cluster_sync();
+            const int first = team + (list + 1 - kept) * teams;
+            for (int e = rank * THREADS + tid; e < kept * wr * 16 * rows; e += ks * THREADS) {
+                const int in = e % (16 * rows), at = e / (16 * rows);
+                const int n = ((first + at / wr * teams) * wr + at % wr) * 16 + (in & 15);
+                float y = 0.0f;
+                for (int x = 0; x < ks; x++) y += peer_load(part + e, uint32_t(x));
+                if (n < a.n) finish(in >> 4, n, y);
+            }
+            cluster_sync();
+            kept = 0;
+        }
     }
-    copy_wait<0>();
 }
 
 template <class XT, int CT, int BPG, bool ZEROS>
 cudaError_t start(Q4Args a, cudaStream_t stream) {
-    constexpr int PARTS = Enter<XT>::PARTS, COLS = 8 * CT;
-    constexpr int X_BYTES = x_bytes_of(CT), FIXED = WARPS * RING + 2 * WARPS * 16 * COLS * 4;
-    const cudaError_t e = raise_shared<q4_kernel<XT, CT, BPG, ZEROS>>(FIXED + X_BYTES);
+    using Q = Q4Tile<CT, BPG, ZEROS>;
+    constexpr int PARTS = Enter<XT>::PARTS;
+    const cudaError_t e = raise_shared<q4_kernel<XT, CT, BPG, ZEROS>>(Q::FIXED + Q::X_BYTES + Q::PART_BYTES);
     if (e != cudaSuccess) return e;
-    a.cols_rows = COLS / PARTS < a.m ? COLS / PARTS : a.m;
-    const int passes = (a.m + a.cols_rows - 1) / a.cols_rows;
-    // chunks of whole turns: a step of x takes 256 bytes a column
-    const int fit = X_BYTES / (256 * a.cols_rows * PARTS);
-    a.chunk_steps = fit >= a.steps ? a.steps : fit / a.wk * a.wk;
-    const int x_bytes = a.chunk_steps * 256 * a.cols_rows * PARTS;
-    const int wr = WARPS / a.wk, lists = ((a.n + 15) / 16 + wr - 1) / wr;
+    CUtensorMap map{};
+    if (a.w_vec) {
+        const EncodeTiled encode = tensor_map_encoder();
+        const cuuint64_t dims[2] = {cuuint64_t(a.k + 1) / 2, cuuint64_t(a.n)}, strides[1] = {cuuint64_t(a.w_row)};
+        const cuuint32_t box[2] = {ROW, 16}, each[2] = {1, 1};
+        a.w_vec = encode && encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(a.w), dims, strides, box, each,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    a.cols_rows = Q::COLS / PARTS < a.m ? Q::COLS / PARTS : a.m;
+    const int passes = (a.m + a.cols_rows - 1) / a.cols_rows, tiles = (a.n + 15) / 16;
+    const int step_bytes = BLOCKS * 64 * (CT == 1 ? a.cols_rows * PARTS : Q::COLS), fit = Q::X_BYTES / step_bytes;
     const int most = sm_count() * (CT <= 2 ? 2 : 1);
-    q4_kernel<XT, CT, BPG, ZEROS><<<dim3(unsigned(lists < most ? lists : most), unsigned(passes)), THREADS, FIXED + x_bytes, stream>>>(a);
-    return cudaGetLastError();
+    a.steps = (a.k + STEP - 1) / STEP;
+    // split k over a cluster's blocks until each one's share of x fits, or
+    // (few tiles) the card is full and each warp has one step
+    a.ks = 1;
+    while (a.ks < 8 && a.steps > a.ks && (a.steps > fit * a.ks || (a.steps >= 2 * a.ks && tiles * a.ks * 2 <= most))) a.ks *= 2;
+    a.share_steps = (a.steps + a.ks - 1) / a.ks;
+    a.wk = 1;
+    while (a.wk < WARPS && a.wk * 2 <= a.share_steps && a.wk * 2 <= fit) a.wk *= 2;
+    // chunks of whole turns where even a share of x is too much
+    a.chunk_steps = fit >= a.share_steps ? a.share_steps : fit / a.wk * a.wk;
+    const int wr = WARPS / a.wk, lists = (tiles + wr - 1) / wr;
+    a.keep = Q::PART_BYTES / (wr * 16 * a.cols_rows * 4);
+    int teams = most / a.ks;
+    teams = lists < teams ? lists : teams;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(unsigned(teams * a.ks), unsigned(passes));
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = Q::FIXED + a.chunk_steps * step_bytes + (a.ks > 1 ? Q::PART_BYTES : 0);
+    c.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(a.ks);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = a.ks > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, q4_kernel<XT, CT, BPG, ZEROS>, a, map);
 }
 
 template <class XT, int CT>
@@ -447,9 +592,6 @@ extern "C" int ppocr_matvec_q4(const ppocr_matvec_q4_shape *s, const void *x, co
     a.scale_type = s->scale_type, a.y_type = s->y_type;
     // one group in all is the row's scale
     a.x_groups = !x_scales ? 0 : s->x_group ? int(groups) : 1;
-    a.steps = (a.k + STEP - 1) / STEP;
-    a.wk = 1;
-    while (a.wk < WARPS && a.wk * 2 <= a.steps) a.wk *= 2;
     a.w_vec = aligned(w, 16) && a.w_row % 16 == 0;
     a.x_vec = uint64_t(a.x_row) * xs % (xs == 1 ? 8 : 16) == 0 && aligned(x, xs == 1 ? 8 : 16);
     const auto str = static_cast<cudaStream_t>(stream);

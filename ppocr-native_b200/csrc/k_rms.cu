@@ -4,14 +4,14 @@
 //     s = x + r;  n = s * rsqrt(mean(s^2) + eps) * gamma
 //     scale_g = max |n| over group g / 448;  y = e4m3(n / scale_g)
 //
-// A row lies in the registers of its threads (8 consecutive channels a
-// chunk, up to four chunks a thread), so x and r are read once and nothing
-// is read again: s leaves rounded to the type, the norm uses the f32 s. The
+// A row lies in the registers of its threads (8 channels a chunk, up to
+// four chunks a thread), so x and r are read once and nothing is read again: s leaves rounded to the type, the norm uses the f32 s. The
 // sum of squares is kept in f32: lane sums, a shuffle tree, then the warps'
 // sums in order (the same order every time). Bound by HBM bytes.
 #include <cuda_fp8.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "block.cuh"
 
@@ -30,72 +30,141 @@ struct RmsArgs {
     float eps;
 };
 
+// A lane's 8 channels of one chunk as they lie in memory.
 template <class T>
-__device__ __forceinline__ void load8(const T *p, int n, bool vec, float v[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4 *>(p)), b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+struct Eight {
+    static constexpr int W = sizeof(T) == 4 ? 2 : 1;
+    uint4 u[W];
+
+    // from 8 consecutive channels at a 16-byte border
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint16_t lo = uint16_t(u[i] & 0xffff), hi = uint16_t(u[i] >> 16);
-                v[2 * i] = to_f32(*reinterpret_cast<const T *>(&lo));
-                v[2 * i + 1] = to_f32(*reinterpret_cast<const T *>(&hi));
+        for (int i = 0; i < W; i++) u[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    // from channels 32 apart, n of the run left from p on
+    __device__ __forceinline__ void load_apart(const T *p, int n) {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(u);
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = i * 32 < n ? __float_as_uint(p[i * 32]) : 0;
+        } else {
+            uint32_t *w = reinterpret_cast<uint32_t *>(u);
+            const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[i] = i * 32 < n ? q[i * 32] : 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = h[2 * i] | h[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void get(float v[8]) const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(u);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+                v[i + 4] = __uint_as_float(w[i + 4]);
+            } else if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < n ? to_f32(p[i]) : 0.0f;
     }
-}
-
-template <class T>
-__device__ __forceinline__ void store8(T *p, int n, bool vec, const float v[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(p) =
-                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    __device__ __forceinline__ void put(const float v[8]) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(u);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = __float_as_uint(v[i]);
+                w[i + 4] = __float_as_uint(v[i + 4]);
+            } else {
+                w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+            }
         }
-    } else {
+    }
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < W; i++) reinterpret_cast<uint4 *>(p)[i] = u[i];
+    }
+    __device__ __forceinline__ void store_apart(T *p, int n) const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(u);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (i < n) p[i] = from_f32<T>(v[i]);
+            if (i * 32 < n) {
+                if constexpr (sizeof(T) == 4)
+                    p[i * 32] = __uint_as_float(w[i]);
+                else
+                    reinterpret_cast<unsigned short *>(p)[i * 32] = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
+            }
     }
-}
+};
 
 // |v| as bits: as integers they order as the magnitudes do, infinity above
 // every number and NaN above infinity, so a NaN is never lost.
 __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// What a group of this peak magnitude is multiplied by for its 8 bits, one
+// over its scale. The scale is rounded to f32 (and may fall to zero), so the
+// quotient by it is taken where 448 / peak would overflow; zero for zeros.
+__device__ __forceinline__ float steps_of(uint32_t peak) {
+    const float p = __uint_as_float(peak);
+    if (p < 1e-30f) return p / 448.0f == 0.0f ? 0.0f : fminf(1.0f / (p / 448.0f), 3e38f);
+    return 448.0f / p;
+}
+
+// Two values as e4m3, the first in the low byte.
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
 // TPR threads a row, CH chunks of 8 channels a thread. Rows narrower than a
-// warp's reach share a block of 128 threads, four rows to it.
+// warp's reach share a block of 128 threads, four rows to it. A block walks
+// rows gridDim apart and has the next row's loads in flight while it works
+// on this one.
+//
+// VEC: a chunk is 8 consecutive channels, 16-byte loads; else (rows, strides
+// or bases that 16 bytes do not divide) channels 32 apart, so that a warp's
+// loads lie side by side.
 template <class T, int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const __grid_constant__ RmsArgs a) {
     constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, WARPS = TPR / 32;
     __shared__ float part[WARPS];
     __shared__ uint32_t peak[WARPS];
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = t / 32;
-    for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < a.rows; row0 += int64_t(gridDim.x) * ROWS) {
-        const int64_t row = row0 + threadIdx.x / TPR;
-        const bool live = row < a.rows;
-        float s[CH][8], square = 0.0f;
-        const T *x = static_cast<const T *>(a.x) + row * a.x_row, *r = static_cast<const T *>(a.r) + row * a.r_row;
-        T *sum = static_cast<T *>(a.sum) + row * a.sum_row;
+    const auto place = [&](int c) { return VEC ? (c * TPR + t) * 8 : (c * TPR + (t & ~31)) * 8 + lane; };
+    const T *x = static_cast<const T *>(a.x), *r = static_cast<const T *>(a.r);
+    Eight<T> nx[CH], nr[CH];
+    const auto fetch = [&](int64_t row) {
+        if (row >= a.rows) return;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int at = (c * TPR + t) * 8, n = live ? min(8, a.channels - at) : 0;
-            const bool vec = VEC && n == 8;
-            if (n > 0) {
-                load8<T>(x + at, n, vec, s[c]);
-                if (a.r) {
+            const int at = place(c);
+            if constexpr (VEC) {
+                if (at < a.channels) {
+                    nx[c].load(x + row * a.x_row + at);
+                    if (r) nr[c].load(r + row * a.r_row + at);
+                }
+            } else {
+                nx[c].load_apart(x + row * a.x_row + at, a.channels - at);
+                if (r) nr[c].load_apart(r + row * a.r_row + at, a.channels - at);
+            }
+        }
+    };
+    int64_t row = int64_t(blockIdx.x) * ROWS + threadIdx.x / TPR;
+    fetch(row);
+    for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < a.rows; row0 += int64_t(gridDim.x) * ROWS) {
+        const int channels = row < a.rows ? a.channels : 0;  // of this row: none past the last
+        float s[CH][8], square = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            if (place(c) < channels) {
+                nx[c].get(s[c]);
+                if (r) {
                     float v[8];
-                    load8<T>(r + at, n, vec, v);
+                    nr[c].get(v);
 #pragma unroll
                     for (int i = 0; i < 8; i++) s[c][i] += v[i];
                 }
@@ -104,35 +173,60 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
                 for (int i = 0; i < 8; i++) s[c][i] = 0.0f;
             }
         }
+        fetch(row + int64_t(gridDim.x) * ROWS);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int at = (c * TPR + t) * 8, n = live ? min(8, a.channels - at) : 0;
-            if (a.sum && n > 0) store8<T>(sum + at, n, VEC && n == 8, s[c]);
 #pragma unroll
             for (int i = 0; i < 8; i++) square = fmaf(s[c][i], s[c][i], square);
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
         if constexpr (WARPS > 1) {
-            __syncthreads();  // the row before is done with part and peak
             if (lane == 0) part[warp] = square;
             __syncthreads();
             square = 0.0f;
 #pragma unroll
             for (int w = 0; w < WARPS; w++) square += part[w];
         }
+        if (a.sum) {
+            T *sum = static_cast<T *>(a.sum) + row * a.sum_row;
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                if (place(c) >= channels) continue;
+                Eight<T> e;
+                e.put(s[c]);
+                if constexpr (VEC)
+                    e.store(sum + place(c));
+                else
+                    e.store_apart(sum + place(c), channels - place(c));
+            }
+        }
         const float inv = 1.0f / sqrtf(square / float(a.channels) + a.eps);
-        uint32_t top[CH], all = 0;
+        uint32_t top[CH][VEC ? 1 : 8], all = 0;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int at = (c * TPR + t) * 8;
-            top[c] = 0;
+            const int at = place(c);
+            if constexpr (VEC) {
+                top[c][0] = 0;
+                if (at < channels) {
+                    const float4 g0 = __ldg(reinterpret_cast<const float4 *>(a.gamma + at));
+                    const float4 g1 = __ldg(reinterpret_cast<const float4 *>(a.gamma + at) + 1);
+                    const float gamma[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                s[c][i] = at + i < a.channels ? s[c][i] * inv * __ldg(a.gamma + at + i) : 0.0f;
-                top[c] = max(top[c], mag(s[c][i]));
+                    for (int i = 0; i < 8; i++) {
+                        s[c][i] = s[c][i] * inv * gamma[i];
+                        top[c][0] = max(top[c][0], mag(s[c][i]));
+                    }
+                }
+                all = max(all, top[c][0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    s[c][i] = at + i * 32 < channels ? s[c][i] * inv * __ldg(a.gamma + at + i * 32) : 0.0f;
+                    top[c][i] = mag(s[c][i]);
+                    all = max(all, top[c][i]);
+                }
             }
-            all = max(all, top[c]);
         }
         float *scales = a.scales + row * a.groups;
         if (a.group == 0) {
@@ -144,41 +238,61 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
 #pragma unroll
                 for (int w = 0; w < WARPS; w++) all = max(all, peak[w]);
             }
-            if (live && t == 0) scales[0] = __uint_as_float(all) / 448.0f;
-#pragma unroll
-            for (int c = 0; c < CH; c++) top[c] = all;
+            if (channels && t == 0) scales[0] = __uint_as_float(all) / 448.0f;
         } else {
-            // a group of 32, 64 or 128 channels is 4, 8 or 16 neighbouring lanes' chunks
 #pragma unroll
             for (int c = 0; c < CH; c++) {
-                top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], 1));
-                top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], 2));
-                if (a.group > 32) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-                if (a.group > 64) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-                const int at = (c * TPR + t) * 8;
-                if (live && at < a.channels && at % a.group == 0) scales[at / a.group] = __uint_as_float(top[c]) / 448.0f;
+                if constexpr (VEC) {
+                    // a group of 32, 64 or 128 channels is 4, 8 or 16 neighbouring lanes' chunks
+                    uint32_t &m = top[c][0];
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    if (a.group > 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    if (a.group > 64) m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    if (place(c) < channels && (place(c) & (a.group - 1)) == 0)
+                        scales[place(c) / a.group] = __uint_as_float(m) / 448.0f;
+                } else {
+                    // 1, 2 or 4 of the warp's 32-channel runs
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top[c][i] = __reduce_max_sync(0xffffffffu, top[c][i]);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2)
+                        if (a.group > 32) top[c][i] = top[c][i + 1] = max(top[c][i], top[c][i + 1]);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4)
+                        if (a.group > 64) top[c][i] = top[c][i + 1] = top[c][i + 2] = top[c][i + 3] = max(top[c][i], top[c][i + 2]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int at = place(c) + i * 32;
+                        if (lane == 0 && at < channels && (at & (a.group - 1)) == 0)
+                            scales[at / a.group] = __uint_as_float(top[c][i]) / 448.0f;
+                    }
+                }
             }
         }
         uint8_t *y = a.y + row * a.y_row;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int at = (c * TPR + t) * 8, n = live ? min(8, a.channels - at) : 0;
-            const float scale = __uint_as_float(top[c]) / 448.0f;
-            uint32_t packed[2] = {0, 0};
+            const int n = channels - place(c);
+            if constexpr (VEC) {
+                if (n <= 0) continue;
+                const float f = steps_of(a.group ? top[c][0] : all);
+                uint32_t w[2];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                // a scale of zero (all zeros, or too small for f32): zeros
-                const float v = scale == 0.0f ? 0.0f : s[c][i] / scale;
-                packed[i / 4] |= uint32_t(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3)) << (8 * (i % 4));
-            }
-            if (VEC && n == 8) {
-                *reinterpret_cast<uint2 *>(y + at) = make_uint2(packed[0], packed[1]);
+                for (int i = 0; i < 2; i++)
+                    w[i] = e4m3_pair(s[c][4 * i] * f, s[c][4 * i + 1] * f) |
+                           e4m3_pair(s[c][4 * i + 2] * f, s[c][4 * i + 3] * f) << 16;
+                *reinterpret_cast<uint2 *>(y + place(c)) = make_uint2(w[0], w[1]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (i < n) y[at + i] = uint8_t(packed[i / 4] >> (8 * (i % 4)));
+                    if (i * 32 < n) y[place(c) + i * 32] = uint8_t(e4m3_pair(s[c][i] * steps_of(a.group ? top[c][i] : all), 0.0f));
             }
         }
+        // the next row's sums go where every warp has read this one's by now:
+        // between two uses of `part`, and of `peak`, lies a barrier of the other
+        if (WARPS > 1 && a.group != 0) __syncthreads();
+        row += int64_t(gridDim.x) * ROWS;
     }
 }
 
@@ -253,7 +367,7 @@ extern "C" int ppocr_rms_norm_e4m3(const ppocr_rms_norm_shape *s, const void *x,
         overlap(scales, cn, x, xn) || overlap(scales, cn, residual, rn) || overlap(scales, cn, gamma, gn))
         return refuse(PPOCR_E_ARG, me, "an output overlaps another buffer");
     const auto wide = [&](const void *p, int64_t row) { return !p || (aligned(p, 16) && uint64_t(row) * size % 16 == 0); };
-    const bool vec = wide(x, a.x_row) && wide(residual, a.r_row) && wide(sum, a.sum_row) && aligned(y, 8) && a.y_row % 8 == 0;
+    const bool vec = c % 8 == 0 && aligned(gamma, 16) && wide(x, a.x_row) && wide(residual, a.r_row) && wide(sum, a.sum_row) && aligned(y, 8) && a.y_row % 8 == 0;
     const auto str = static_cast<cudaStream_t>(stream);
     const cudaError_t e = s->type == PPOCR_F32   ? start_t<float>(a, vec, str)
                           : s->type == PPOCR_F16 ? start_t<__half>(a, vec, str)
