@@ -203,7 +203,7 @@ typedef struct {
     uint32_t head_dim;                       /* 1 to 128 */
     int32_t left, right;                     /* keys seen before and behind the query's own; -1: no limit */
     uint32_t sinks;                          /* a lane's first keys, seen however far back they are */
-    float scale;                             /* of the scores */
+    float scale;                             /* of the scores, not negative */
     uint32_t max_q, max_k;                   /* about the longest lane's queries and keys (0: unknown); they size
                                                 the launch, never the result */
     uint64_t q_rows, kv_rows;                /* rows q and out, and k and v, hold (at most 2^30) */

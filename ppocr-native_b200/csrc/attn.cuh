@@ -24,9 +24,9 @@ struct AttnArgs {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
     int lanes, heads, kv_heads, share, d;
     int left, right, sinks;  // left, right -1: no limit
-    float scale, scale_log2;
+    float scale_log2;  // the scale times log2 e
     int q_bytes, k_bytes, v_bytes;  // widest copy each tensor's rows allow: 16, 4 or 2 bytes
-    int out_vec;                     // 1 when pairs of outputs may be stored together
+    int out_vec;                     // 1 when pairs of outputs may be stored together, 2 when 16 bytes may
 };
 
 namespace {
@@ -323,6 +323,8 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
 // Each returns a CUDA error; the grid covers any lane lengths, the hints
 // only size it.
 cudaError_t launch_attn_rows(const AttnArgs &a, int type, uint32_t max_q, cudaStream_t stream);
+// *taken says whether this form takes the call (types, alignment).
+cudaError_t launch_attn_tc(const AttnArgs &a, int type, uint32_t max_q, bool *taken, cudaStream_t stream);
 cudaError_t launch_attn_split(const AttnArgs &a, int type, uint32_t max_q, uint32_t max_keys, cudaStream_t stream);
 
 }  // namespace ppocr

@@ -178,7 +178,7 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     if (!s->heads || !s->kv_heads || s->heads % s->kv_heads)
         return refuse(PPOCR_E_ARG, me, "heads must be a multiple of kv_heads");
     if (s->left < -1 || s->right < -1) return refuse(PPOCR_E_ARG, me, "left and right are -1 (no limit) or more");
-    if (!std::isfinite(s->scale)) return refuse(PPOCR_E_ARG, me, "scale is not finite");
+    if (!std::isfinite(s->scale) || s->scale < 0.0f) return refuse(PPOCR_E_ARG, me, "scale must be finite and not negative");
     if (!s->head_dim || s->head_dim > 128) return refuse(PPOCR_E_SIZE, me, "head_dim must be between 1 and 128");
     if (s->heads > 65535 || s->lanes > 65535) return refuse(PPOCR_E_SIZE, me, "more than 65535 heads or lanes");
     const uint64_t most = uint64_t(1) << 40, rows_most = uint64_t(1) << 30;
@@ -223,12 +223,13 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     a.left = s->left, a.right = s->right < far ? s->right : far;
     a.left = a.left < far ? a.left : far;
     a.sinks = int(s->sinks < uint32_t(far) ? s->sinks : uint32_t(far));
-    a.scale = s->scale;
+    // a scale of zero would turn a hidden score's minus infinity into NaN
     a.scale_log2 = s->scale * 1.4426950408889634f;
+    if (a.scale_log2 < 1.2e-38f) a.scale_log2 = 1.2e-38f;
     a.q_bytes = copy_bytes(q, s->q_row, s->q_head, size);
     a.k_bytes = copy_bytes(k, s->k_row, s->k_head, size);
     a.v_bytes = copy_bytes(v, s->v_row, s->v_head, size);
-    a.out_vec = (reinterpret_cast<uintptr_t>(out) | s->out_row * size | s->out_head * size) % (2 * size) == 0;
+    a.out_vec = copy_bytes(out, s->out_row, s->out_head, size) == 16 ? 2 : (reinterpret_cast<uintptr_t>(out) | s->out_row * size | s->out_head * size) % (2 * size) == 0 ? 1 : 0;
 
     const uint32_t max_q = s->max_q ? uint32_t(s->max_q < s->q_rows ? s->max_q : s->q_rows) : uint32_t(s->q_rows);
     uint64_t keys = s->max_k && s->max_k < s->kv_rows ? s->max_k : s->kv_rows;
@@ -238,8 +239,12 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     }
     const auto str = static_cast<cudaStream_t>(stream);
     // few query rows a key head (single steps): the keys are split instead
-    const cudaError_t e = uint64_t(max_q) * a.share <= 16
-                              ? launch_attn_split(a, s->type, max_q, uint32_t(keys), str)
-                              : launch_attn_rows(a, s->type, max_q, str);
+    if (uint64_t(max_q) * a.share <= 16) {
+        const cudaError_t e = launch_attn_split(a, s->type, max_q, uint32_t(keys), str);
+        return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
+    }
+    bool taken = false;
+    cudaError_t e = launch_attn_tc(a, s->type, max_q, &taken, str);
+    if (!taken) e = launch_attn_rows(a, s->type, max_q, str);
     return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
 }

@@ -1,0 +1,371 @@
+// Window attention over whole lanes on the 5th-generation tensor cores (f16
+// and bf16, rows and heads on 16-byte borders).
+//
+// A block takes 128 queries of one head (a thread a row) and walks the key
+// tiles they see: the sinks, then up to 128 keys at a time from the window's
+// first key on, the last tile in steps of 16. Per tile:
+//     S = Q K^T      tcgen05.mma, Q and K in shared memory (TMA, 128-byte
+//                    swizzle), S in tensor memory
+//     softmax        four warps: a row's 128 scores in registers, P back into
+//                    S's place in 16 bits
+//     O += P V       tcgen05.mma, P from tensor memory, V as it lies in shared
+//                    memory (its head dimension is the instruction's N)
+// One thread issues copies and products. Two blocks share an SM (256 columns
+// of tensor memory and 96 KB of shared memory each), so that one's products
+// run under the other's softmax; inside a block the steps follow one another
+// and nothing needs a second buffer: K is refilled under the softmax, V under
+// the next product.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since
+// the last time (the weights stay below 2^8, their sums in f32), which is rare
+// after the first tile. Bound by the exponentials (16 a cycle and SM) and the
+// products (1024 cycles a tile of 128 keys at head size 128) alike.
+#include <type_traits>
+
+#include "attn.cuh"
+
+namespace ppocr {
+
+namespace {
+
+constexpr int BQ = 128, BK = 128, SOFTMAX_WARPS = 4, THREADS = SOFTMAX_WARPS * 32 + 32;
+constexpr int BOX = 32;                    // rows a copy brings: 4 KB of one 64-column panel
+constexpr int BOX_BYTES = BOX * 128;
+constexpr int TMEM_COLS = 256;             // S (and P in its place): 0 to 127, O: 128 to 255
+constexpr int O_COL = 128;
+constexpr float GROW = 8.0f;               // log2 of how far a maximum may grow before O is rescaled
+
+struct Maps {
+    CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    // shared-memory matrix descriptor: start, leading and stride offsets in
+    // 16-byte units, version 1, 128-byte swizzle (2)
+    return uint64_t((addr >> 4) & 0x3FFF) | uint64_t((lead >> 4) & 0x3FFF) << 16 | uint64_t((stride >> 4) & 0x3FFF) << 32 |
+           uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+
+// kind::f16: D f32, A and B f16 (0) or bf16 (1), M = 128, N = n; B's major
+// dimension: 0 k, 1 n.
+template <class T>
+__device__ __forceinline__ uint32_t idesc(int n, int b_major) {
+    constexpr uint32_t F = std::is_same<T, __half>::value ? 0 : 1;
+    return (1u << 4) | (F << 7) | (F << 10) | (uint32_t(b_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(BQ >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float *v) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// The tiles of one query tile: the sinks below the window, then the window.
+struct Tiles {
+    int sink_end, lo, hi, n_sink, n;
+    __device__ __forceinline__ Tiles(const AttnArgs &a, int p0, int p1, int nk) {
+        hi = max(0, a.right < 0 ? nk : min(nk, p1 + a.right + 1));
+        lo = a.left < 0 ? 0 : min(max(0, p0 - a.left), hi);
+        sink_end = min(a.sinks, lo);
+        n_sink = (sink_end + BK - 1) / BK;
+        n = n_sink + (hi - lo + BK - 1) / BK;
+    }
+    __device__ __forceinline__ int first(int it) const { return it < n_sink ? it * BK : lo + (it - n_sink) * BK; }
+    __device__ __forceinline__ int count(int it) const {
+        return it < n_sink ? min(BK, sink_end - it * BK) : min(BK, hi - lo - (it - n_sink) * BK);
+    }
+};
+
+template <class T>
+__global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t bars[6];  // Q, K and V have come; S is done; P is there; O is done
+    __shared__ uint32_t tmem_s;
+    __shared__ int give_up_s;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int panels = (a.d + 63) / 64, dn = (a.d + 15) / 16 * 16;  // 64-column panels; head size in steps of 16
+    const uint32_t q_s = shared_u32(smem), k_s = q_s + panels * (BQ * 128), v_s = k_s + panels * (BK * 128);
+    const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 16, s_bar = q_bar + 24, p_bar = q_bar + 32,
+                   o_bar = q_bar + 40;
+    volatile int *give_up = &give_up_s;
+    if (tid == 0) {
+        for (int i = 0; i < 6; i++) bar_init(q_bar + 8 * i, i == 4 ? SOFTMAX_WARPS : 1);
+        give_up_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == SOFTMAX_WARPS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_u32(&tmem_s)), "r"(TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_s;
+    // a wait that ran out of time ends every role's; the rows are done again the plain way
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (*give_up) return false;
+        if (wait_copy(bar, parity)) return true;
+        *give_up = 1;
+        return false;
+    };
+
+    const Lane ln = read_lane(a, blockIdx.z);
+    const int h = blockIdx.y, kvh = h / a.share;
+    uint32_t turn = 0, tile_turn = 0;  // query tiles and key tiles so far: the barriers' phases
+    for (int64_t i0 = int64_t(blockIdx.x) * BQ; i0 < ln.nq; i0 += int64_t(gridDim.x) * BQ, turn++) {
+        const int rows = int(ln.nq - i0 < BQ ? ln.nq - i0 : BQ);
+        const int p0 = int(i0) + ln.nk - ln.nq;
+        const Tiles tl(a, p0, p0 + rows - 1, ln.nk);
+        if (warp == SOFTMAX_WARPS) {
+            if (lane == 0 && tl.n > 0) {
+                const auto load = [&](const CUtensorMap *map, uint32_t to, int head, int64_t row, int n, uint32_t bar) {
+                    const int boxes = (n + BOX - 1) / BOX;
+                    arrive_expect(bar, uint32_t(boxes * panels * BOX_BYTES));
+                    for (int p = 0; p < panels; p++)
+                        for (int b = 0; b < boxes; b++)
+                            tma_load_3d(to + uint32_t(p * (BK * 128) + b * BOX_BYTES), map, p * 64, head, int(row) + b * BOX, bar);
+                };
+                load(&maps.q, q_s, h, ln.q0 + i0, rows, q_bar);
+                load(&maps.k, k_s, kvh, ln.k0 + tl.first(0), tl.count(0), k_bar);
+                load(&maps.v, v_s, kvh, ln.k0 + tl.first(0), tl.count(0), v_bar);
+                bool on = wait(q_bar, turn & 1);
+                for (int it = 0; on && it < tl.n; it++) {
+                    const uint32_t par = (tile_turn + it) & 1;
+                    const int n = (tl.count(it) + 15) / 16 * 16;
+                    if (!(on = wait(k_bar, par))) break;
+                    fence_after();
+                    const uint32_t id_s = idesc<T>(n, 0);
+                    for (int kk = 0; kk < dn / 16; kk++) {
+                        const uint32_t at = uint32_t((kk >> 2) * (BK * 128) + (kk & 3) * 32);
+                        mma_ss(tmem, desc(q_s + at, 16, 1024), desc(k_s + at, 16, 1024), id_s, kk > 0);
+                    }
+                    commit(s_bar);
+                    if (!(on = wait(s_bar, par))) break;  // K is read
+                    if (it + 1 < tl.n) load(&maps.k, k_s, kvh, ln.k0 + tl.first(it + 1), tl.count(it + 1), k_bar);
+                    if (!(on = wait(v_bar, par) && wait(p_bar, par))) break;
+                    fence_after();
+                    const uint32_t id_o = idesc<T>(dn, 1);
+                    for (int kk = 0; kk < n / 16; kk++)
+                        mma_ts(tmem + O_COL, tmem + kk * 8, desc(v_s + uint32_t(kk * 2048), BK * 128, 1024), id_o, it > 0 || kk > 0);
+                    commit(o_bar);
+                    if (!(on = wait(o_bar, par))) break;  // V and P are read
+                    if (it + 1 < tl.n) load(&maps.v, v_s, kvh, ln.k0 + tl.first(it + 1), tl.count(it + 1), v_bar);
+                }
+            }
+            __syncwarp();
+        } else {
+            const int row = warp * 32 + lane, p = p0 + row;
+            const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int it = 0; it < tl.n; it++) {
+                const uint32_t par = (tile_turn + it) & 1;
+                const int j0 = tl.first(it), n = tl.count(it);
+                ok = wait(s_bar, par);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+                float s[BK];
+#pragma unroll
+                for (int c = 0; c < BK / 32; c++) tmem_load32(mine + c * 32, s + c * 32);
+                tmem_wait_load();
+                // this row's keys of the tile: a run, and below the sinks' end all
+                // that the right side leaves
+                const bool whole = n == BK && (a.right < 0 || j0 + BK - 1 <= p0 + warp * 32 + a.right) &&
+                                   (a.left < 0 || j0 >= p0 + warp * 32 + 31 - a.left || j0 + BK <= a.sinks);
+                if (!whole) {
+                    const int end = a.right < 0 ? n : max(0, min(n, p + a.right + 1 - j0));
+                    const int from = a.left < 0 ? 0 : max(0, p - a.left - j0), sunk = a.sinks - j0;
+#pragma unroll
+                    for (int j = 0; j < BK; j++)
+                        if (j >= end || (j < from && j >= sunk)) s[j] = -INFINITY;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < BK; j += 8)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) top[x] = fmaxf(fmaxf(top[x], s[j + x]), s[j + 4 + x]);
+                const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                // O's row is zero while no key was seen: nothing to rescale then
+                float keep = 1.0f;
+                if (now > m + GROW || m == -INFINITY) {
+                    keep = m == -INFINITY ? 1.0f : exp2_fast(m - now);
+                    m = now;
+                }
+                if (__any_sync(0xffffffffu, keep != 1.0f)) {
+                    l *= keep;
+                    for (int c = 0; c < dn; c += 16) {
+                        float o[16];
+                        uint32_t *r = reinterpret_cast<uint32_t *>(o);
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                            : "r"(mine + O_COL + c));
+                        tmem_wait_load();
+#pragma unroll
+                        for (int x = 0; x < 16; x++) o[x] *= keep;
+                        tmem_store16(mine + O_COL + c, r);
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < BK / 32; c++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const float e0 = exp2_fast(fmaf(s[c * 32 + 2 * x], a.scale_log2, -base));
+                        const float e1 = exp2_fast(fmaf(s[c * 32 + 2 * x + 1], a.scale_log2, -base));
+                        sum[x & 1] += e0;
+                        sum[2 + (x & 1)] += e1;
+                        w[x] = pack2<T>(e0, e1);
+                    }
+                    tmem_store16(mine + c * 16, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                // rows of V past the lane's keys, up to the product's step of 16:
+                // whatever lies there, zero
+                if (n & 15) {
+                    ok = wait(v_bar, par);
+                    const int gap = 16 - (n & 15);
+                    for (int e = row; e < gap * panels * 8; e += SOFTMAX_WARPS * 32) {
+                        const int r = n + e / (panels * 8), c = e % (panels * 8);
+                        *reinterpret_cast<uint4 *>(smem + (v_s - q_s) + (c >> 3) * (BK * 128) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(p_bar);
+            }
+            if (tl.n > 0 && ok) ok = wait(o_bar, (tile_turn + tl.n - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            fence_after();
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            bool bad = !ok || !(l < INFINITY);
+            T *out = static_cast<T *>(a.out) + (ln.q0 + i0 + row) * a.out_row + h * a.out_head;
+            if (ok) {
+                for (int c = 0; c < dn; c += 16) {
+                    float o[16];
+                    uint32_t *r = reinterpret_cast<uint32_t *>(o);
+                    asm volatile(
+                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                        : "r"(mine + O_COL + c));
+                    tmem_wait_load();
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        o[x] = tl.n == 0 ? 0.0f : o[x] * inv;  // no tile: O was never written
+                        bad |= !(fabsf(o[x]) < INFINITY);
+                    }
+                    if (row < rows) {
+                        if (a.out_vec == 2 && c + 16 <= a.d) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int x = 0; x < 8; x++) w[x] = pack2<T>(o[2 * x], o[2 * x + 1]);
+                            reinterpret_cast<uint4 *>(out + c)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                            reinterpret_cast<uint4 *>(out + c)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 16; x++)
+                                if (c + x < a.d) out[c + x] = from_f32<T>(o[x]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            unsigned again = __ballot_sync(0xffffffffu, bad && row < rows);
+            while (again) {
+                const int r = __ffs(again) - 1;
+                again &= again - 1;
+                row_alone<T>(a, ln, int(i0) + warp * 32 + r, h);
+            }
+            fence_before();
+        }
+        tile_turn += tl.n;
+        if (tl.n == 0) turn--;
+        __syncthreads();  // O is read: the next query tile's product may overwrite it
+        fence_after();
+        if (*give_up) break;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == SOFTMAX_WARPS) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+    }
+}
+
+bool map_rows(CUtensorMap *map, const void *p, int type, int64_t rows, int64_t row, int heads, int64_t head, int d) {
+    const EncodeTiled encode = tensor_map_encoder();
+    // a single head's stride is never used, but has to be a valid one
+    const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
+    const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head : (d + 7) / 8 * 8) * 2, cuuint64_t(rows > 1 ? row : (d + 7) / 8 * 8) * 2};
+    const cuuint32_t box[3] = {64, 1, BOX}, each[3] = {1, 1, 1};
+    return encode && encode(map, type == PPOCR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                            const_cast<void *>(p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T>
+cudaError_t start(const AttnArgs &a, const Maps &maps, uint32_t max_q, cudaStream_t stream) {
+    const int panels = (a.d + 63) / 64, shared = 3 * panels * BK * 128;
+    const cudaError_t e = raise_shared<attn_tc_kernel<T>>(3 * 2 * BK * 128);
+    if (e != cudaSuccess) return e;
+    const uint32_t tiles = max_q ? (max_q + BQ - 1) / BQ : 1;
+    attn_tc_kernel<T><<<dim3(tiles, unsigned(a.heads), unsigned(a.lanes)), THREADS, shared, stream>>>(a, maps);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tc(const AttnArgs &a, int type, uint32_t max_q, bool *taken, cudaStream_t stream) {
+    *taken = false;
+    if (type == PPOCR_F32 || a.q_bytes != 16 || a.k_bytes != 16 || a.v_bytes != 16) return cudaSuccess;
+    Maps maps;
+    if (!map_rows(&maps.q, a.q, type, a.q_rows, a.q_row, a.heads, a.q_head, a.d) ||
+        !map_rows(&maps.k, a.k, type, a.kv_rows, a.k_row, a.kv_heads, a.k_head, a.d) ||
+        !map_rows(&maps.v, a.v, type, a.kv_rows, a.v_row, a.kv_heads, a.v_head, a.d))
+        return cudaSuccess;  // strides the encoder does not take
+    *taken = true;
+    return type == PPOCR_F16 ? start<__half>(a, maps, max_q, stream) : start<__nv_bfloat16>(a, maps, max_q, stream);
+}
+
+}  // namespace ppocr

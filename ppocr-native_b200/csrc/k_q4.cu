@@ -95,18 +95,19 @@ __device__ __forceinline__ float part_of(float x, int part) {
 // which serves every multiple of 32).
 template <int CT>
 struct Q4Tile {
-    static constexpr int COLS = 8 * CT, SL = CT == 1 ? 2 : 1, DEPTH = 4 / SL;
+    // a row of partial sums, padded so that 16 rows' columns lie in different banks
+    static constexpr int COLS = 8 * CT, WIDE = COLS + 2, SL = CT == 1 ? 2 : 1, DEPTH = 4 / SL;
     // 64 registers of x a lane with four column tiles: half the warps
     static constexpr int WARPS = CT == 4 ? 8 : 16;
-    static constexpr int SHARED = (CT == 4 ? 160 : 200) * 1024;
+    static constexpr int SHARED = 200 * 1024;
 };
 
 template <class XT, int CT, int BPG, bool ZEROS>
 __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __grid_constant__ Q4Args a) {
     using M = typename Enter<XT>::M;
     using Q = Q4Tile<CT>;
-    constexpr int PARTS = Enter<XT>::PARTS, COLS = Q::COLS, SL = Q::SL, DEPTH = Q::DEPTH;
-    extern __shared__ __align__(16) float red[];  // [list of the batch][tile of the item][warp][16][COLS], then the cluster's sums
+    constexpr int PARTS = Enter<XT>::PARTS, WIDE = Q::WIDE, SL = Q::SL, DEPTH = Q::DEPTH;
+    extern __shared__ __align__(16) float red[];  // [list of the batch][tile of the item][warp][16][WIDE], then the cluster's sums
     const Place at(a);
     const int warps = int(blockDim.x) / 32;
     const int m0 = blockIdx.y * a.cols_rows, rows = min(a.cols_rows, a.m - m0);
@@ -139,10 +140,10 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
             }
     };
     const auto value = [&](int l, int tile, int m, int r) {
-        const float *from = red + (((l * a.depth + tile % a.depth) * warps + tile / a.depth * a.wk) * 16 + r) * COLS + m * PARTS;
+        const float *from = red + (((l * a.depth + tile % a.depth) * warps + tile / a.depth * a.wk) * 16 + r) * WIDE + m * PARTS;
         float y = 0.0f;
         for (int p = PARTS - 1; p >= 0; p--)
-            for (int w = 0; w < a.wk; w++) y += from[w * 16 * COLS + p];
+            for (int w = 0; w < a.wk; w++) y += from[w * 16 * WIDE + p];
         return y;
     };
     const auto finish = [&](int m, int n, float y) {
@@ -214,12 +215,12 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                         }
                         in.chunk(a, at, d, c);
                     }
-                    float *mine = red + (((i * a.depth + d) * warps + at.warp) * 16 + at.g) * COLS + at.t * 2;
+                    float *mine = red + (((i * a.depth + d) * warps + at.warp) * 16 + at.g) * WIDE + at.t * 2;
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            float2 *to = reinterpret_cast<float2 *>(mine + h * 8 * COLS + ct * 8);
+                            float2 *to = reinterpret_cast<float2 *>(mine + h * 8 * WIDE + ct * 8);
                             float2 v = make_float2(acc[ct][2 * h], acc[ct][2 * h + 1]);
                             if (lap > 0) v.x += to->x, v.y += to->y;
                             *to = v;
@@ -238,7 +239,7 @@ cudaError_t start(Q4Args a, cudaStream_t stream) {
     const cudaError_t e = raise_shared<q4_kernel<XT, CT, BPG, ZEROS>>(Q::SHARED);
     if (e != cudaSuccess) return e;
     a.cols_rows = Q::COLS / Enter<XT>::PARTS < a.m ? Q::COLS / Enter<XT>::PARTS : a.m;
-    return launch_q4(reinterpret_cast<const void *>(q4_kernel<XT, CT, BPG, ZEROS>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, Q::COLS, 0,
+    return launch_q4(reinterpret_cast<const void *>(q4_kernel<XT, CT, BPG, ZEROS>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, Q::WIDE, 0,
                      Q::SHARED, stream);
 }
 

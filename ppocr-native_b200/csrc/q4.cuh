@@ -348,13 +348,15 @@ cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth
     while (a.ks < 8 && a.ks * a.wk < slices) a.ks *= 2;
     a.share = (slices + a.ks - 1) / a.ks * sl;
     a.laps = (a.share + a.wk * sl - 1) / (a.wk * sl);
-    // fewer tiles an item, then fewer items a block, where the card's warps
-    // would not all have one
+    // fewer tiles an item, then fewer items a block, as long as every item still
+    // has a warp, and every block an SM, at once
     const int64_t room = int64_t(sms) * (warps / a.wk) / (passes * a.ks);
-    while (depth > 1 && (a.n + depth * 16 - 1) / (depth * 16) < room) depth /= 2;
+    const auto items_of = [&](int d) { return (a.n + d * 16 - 1) / (d * 16); };
+    while (depth > 1 && items_of(depth / 2) <= room) depth /= 2;
     a.depth = depth;
-    const int items = (a.n + depth * 16 - 1) / (depth * 16);
-    while (warps > a.wk && int64_t(items) * passes * a.ks < int64_t(sms) * (warps / a.wk)) warps /= 2;
+    const int items = items_of(depth);
+    const auto blocks_of = [&](int w) { return int64_t((items + w / a.wk - 1) / (w / a.wk)) * passes * a.ks; };
+    while (warps > a.wk && blocks_of(warps / 2) <= sms) warps /= 2;
     const int wr = warps / a.wk, lists = (items + wr - 1) / wr;
     int teams = sms / a.ks;
     teams = lists < teams ? lists : teams;
