@@ -10,7 +10,7 @@
 //                    S's place in 16 bits
 //     O += P V       tcgen05.mma, P from tensor memory, V as it lies in shared
 //                    memory (its head dimension is the instruction's N)
-// One thread issues copies and products. Two blocks share an SM (256 columns
+// One thread issues the products, one the copies. Two blocks share an SM (256 columns
 // of tensor memory and 96 KB of shared memory each), so that one's products
 // run under the other's softmax; inside a block the steps follow one another
 // and nothing needs a second buffer: K is refilled under the softmax, V under
@@ -23,12 +23,13 @@
 #include <type_traits>
 
 #include "attn.cuh"
+#include "devmath.cuh"
 
 namespace ppocr {
 
 namespace {
 
-constexpr int BQ = 128, BK = 128, SOFTMAX_WARPS = 4, THREADS = SOFTMAX_WARPS * 32 + 32;
+constexpr int BQ = 128, BK = 128, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
 constexpr int BOX = 32;                    // rows a copy brings: 4 KB of one 64-column panel
 constexpr int BOX_BYTES = BOX * 128;
 constexpr int TMEM_COLS = 256;             // S (and P in its place): 0 to 127, O: 128 to 255
@@ -54,18 +55,23 @@ __device__ __forceinline__ uint32_t idesc(int n, int b_major) {
     return (1u << 4) | (F << 7) | (F << 10) | (uint32_t(b_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(BQ >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// Issued where `on` is true: a predicate and no branch, so that the operands
+// stay in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t on) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(on));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t on) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(on));
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t on) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on)
+        : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float *v) {
@@ -79,6 +85,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float *v) {
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float *v) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
@@ -90,6 +104,29 @@ __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// True in one lane of a whole warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, rd;}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// Bits 0 to n - 1.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 // The tiles of one query tile: the sinks below the window, then the window.
 struct Tiles {
@@ -110,47 +147,55 @@ struct Tiles {
 template <class T>
 __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ uint64_t bars[6];  // Q, K and V have come; S is done; P is there; O is done
+    __shared__ uint64_t bars[7];  // Q, K and V have come; S is done; P's halves are there; O is done
     __shared__ uint32_t tmem_s;
     __shared__ int give_up_s;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    // the warp's number and the tensor memory's address by a shuffle, which the
+    // compiler knows to be the same in every lane: the products' operands then
+    // stay in uniform registers (64 cycles a product of 128 x 128 x 16; 110 with
+    // each operand moved there first)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid & 31;
     const int panels = (a.d + 63) / 64, dn = (a.d + 15) / 16 * 16;  // 64-column panels; head size in steps of 16
     const uint32_t q_s = shared_u32(smem), k_s = q_s + panels * (BQ * 128), v_s = k_s + panels * (BK * 128);
-    const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 16, s_bar = q_bar + 24, p_bar = q_bar + 32,
-                   o_bar = q_bar + 40;
+    const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 16, s_bar = q_bar + 24, o_bar = q_bar + 32,
+                   p_bar = q_bar + 40;
     volatile int *give_up = &give_up_s;
     if (tid == 0) {
-        for (int i = 0; i < 6; i++) bar_init(q_bar + 8 * i, i == 4 ? SOFTMAX_WARPS : 1);
+        for (int i = 0; i < 7; i++) bar_init(q_bar + 8 * i, i >= 5 ? SOFTMAX_WARPS : 1);
         give_up_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == SOFTMAX_WARPS) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_u32(&tmem_s)), "r"(TMEM_COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_s;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0);
+    const bool one = elect_one();
     // a wait that ran out of time ends every role's; the rows are done again the plain way
     const auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (*give_up) return false;
-        if (wait_copy(bar, parity)) return true;
+        const bool came = !*give_up && wait_copy(bar, parity);
+        if (__all_sync(0xffffffffu, came)) return true;
         *give_up = 1;
         return false;
     };
 
-    const Lane ln = read_lane(a, blockIdx.z);
+    Lane ln = read_lane(a, blockIdx.z);
+    ln.q0 = __shfl_sync(0xffffffffu, ln.q0, 0), ln.k0 = __shfl_sync(0xffffffffu, ln.k0, 0);
+    ln.nq = __shfl_sync(0xffffffffu, ln.nq, 0), ln.nk = __shfl_sync(0xffffffffu, ln.nk, 0);
     const int h = blockIdx.y, kvh = h / a.share;
     uint32_t turn = 0, tile_turn = 0;  // query tiles and key tiles so far: the barriers' phases
     for (int64_t i0 = int64_t(blockIdx.x) * BQ; i0 < ln.nq; i0 += int64_t(gridDim.x) * BQ, turn++) {
         const int rows = int(ln.nq - i0 < BQ ? ln.nq - i0 : BQ);
         const int p0 = int(i0) + ln.nk - ln.nq;
         const Tiles tl(a, p0, p0 + rows - 1, ln.nk);
-        if (warp == SOFTMAX_WARPS) {
-            if (lane == 0 && tl.n > 0) {
+        if (warp == COPY_WARP) {
+            if (tl.n > 0) {
                 const auto load = [&](const CUtensorMap *map, uint32_t to, int head, int64_t row, int n, uint32_t bar) {
                     const int boxes = (n + BOX - 1) / BOX;
+                    if (!one) return;
                     arrive_expect(bar, uint32_t(boxes * panels * BOX_BYTES));
                     for (int p = 0; p < panels; p++)
                         for (int b = 0; b < boxes; b++)
@@ -159,28 +204,52 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 load(&maps.q, q_s, h, ln.q0 + i0, rows, q_bar);
                 load(&maps.k, k_s, kvh, ln.k0 + tl.first(0), tl.count(0), k_bar);
                 load(&maps.v, v_s, kvh, ln.k0 + tl.first(0), tl.count(0), v_bar);
+                for (int it = 1; it < tl.n; it++) {
+                    const uint32_t before = (tile_turn + it - 1) & 1;
+                    if (!wait(s_bar, before)) break;  // K is read
+                    load(&maps.k, k_s, kvh, ln.k0 + tl.first(it), tl.count(it), k_bar);
+                    if (!wait(o_bar, before)) break;  // V is read
+                    load(&maps.v, v_s, kvh, ln.k0 + tl.first(it), tl.count(it), v_bar);
+                }
+            }
+            __syncwarp();
+        } else if (warp == MMA_WARP) {
+            if (tl.n > 0) {
+                const uint64_t q_desc = desc(q_s, 16, 1024), k_desc = desc(k_s, 16, 1024), v_desc = desc(v_s, BK * 128, 1024);
+                const uint32_t id_o = idesc<T>(dn, 1);
+                const int steps = dn / 16;
+                // no early way out of the loop: its control stays the same in every
+                // lane, and after a wait that ran out no product is issued
                 bool on = wait(q_bar, turn & 1);
-                for (int it = 0; on && it < tl.n; it++) {
+                for (int it = 0; it < tl.n; it++) {
                     const uint32_t par = (tile_turn + it) & 1;
-                    const int n = (tl.count(it) + 15) / 16 * 16;
-                    if (!(on = wait(k_bar, par))) break;
+                    const int n = (tl.count(it) + 15) / 16;
+                    on &= wait(k_bar, par);
                     fence_after();
-                    const uint32_t id_s = idesc<T>(n, 0);
-                    for (int kk = 0; kk < dn / 16; kk++) {
-                        const uint32_t at = uint32_t((kk >> 2) * (BK * 128) + (kk & 3) * 32);
-                        mma_ss(tmem, desc(q_s + at, 16, 1024), desc(k_s + at, 16, 1024), id_s, kk > 0);
+                    const uint32_t id_s = idesc<T>(n * 16, 0);
+                    const uint32_t go = one && on;
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++) {
+                        // the descriptors' addresses count 16 bytes
+                        constexpr uint64_t panel = BK * 128 / 16;
+                        const uint64_t at = (kk >> 2) * panel + (kk & 3) * 2;
+                        mma_ss(tmem, q_desc + at, k_desc + at, id_s, kk > 0, go & uint32_t(kk < steps));
                     }
-                    commit(s_bar);
-                    if (!(on = wait(s_bar, par))) break;  // K is read
-                    if (it + 1 < tl.n) load(&maps.k, k_s, kvh, ln.k0 + tl.first(it + 1), tl.count(it + 1), k_bar);
-                    if (!(on = wait(v_bar, par) && wait(p_bar, par))) break;
+                    commit(s_bar, go);
+                    on &= wait(v_bar, par) && wait(p_bar, par);
                     fence_after();
-                    const uint32_t id_o = idesc<T>(dn, 1);
-                    for (int kk = 0; kk < n / 16; kk++)
-                        mma_ts(tmem + O_COL, tmem + kk * 8, desc(v_s + uint32_t(kk * 2048), BK * 128, 1024), id_o, it > 0 || kk > 0);
-                    commit(o_bar);
-                    if (!(on = wait(o_bar, par))) break;  // V and P are read
-                    if (it + 1 < tl.n) load(&maps.v, v_s, kvh, ln.k0 + tl.first(it + 1), tl.count(it + 1), v_bar);
+                    const uint32_t go1 = one && on;
+#pragma unroll
+                    for (int kk = 0; kk < BK / 32; kk++)
+                        mma_ts(tmem + O_COL, tmem + kk * 8, v_desc + uint64_t(kk * 128), id_o, it > 0 || kk > 0, go1 & uint32_t(kk < n));
+                    on &= wait(p_bar + 8, par);
+                    fence_after();
+                    const uint32_t go2 = one && on;
+#pragma unroll
+                    for (int kk = BK / 32; kk < BK / 16; kk++)
+                        mma_ts(tmem + O_COL, tmem + kk * 8, v_desc + uint64_t(kk * 128), id_o, 1, go2 & uint32_t(kk < n));
+                    commit(o_bar, go2);
+                    on &= wait(o_bar, par);  // S's place is free
                 }
             }
             __syncwarp();
@@ -193,31 +262,35 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 const uint32_t par = (tile_turn + it) & 1;
                 const int j0 = tl.first(it), n = tl.count(it);
                 ok = wait(s_bar, par);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
+                if (!ok) break;
                 fence_after();
                 float s[BK];
 #pragma unroll
-                for (int c = 0; c < BK / 32; c++) tmem_load32(mine + c * 32, s + c * 32);
+                for (int c = 0; c < BK / 32; c++)
+                    if (c * 32 < n) tmem_load32(mine + c * 32, s + c * 32);
                 tmem_wait_load();
                 // this row's keys of the tile: a run, and below the sinks' end all
                 // that the right side leaves
-                const bool whole = n == BK && (a.right < 0 || j0 + BK - 1 <= p0 + warp * 32 + a.right) &&
-                                   (a.left < 0 || j0 >= p0 + warp * 32 + 31 - a.left || j0 + BK <= a.sinks);
+                const bool whole = n % 32 == 0 && (a.right < 0 || j0 + n - 1 <= p0 + warp * 32 + a.right) &&
+                                   (a.left < 0 || j0 >= p0 + warp * 32 + 31 - a.left || j0 + n <= a.sinks);
                 if (!whole) {
-                    const int end = a.right < 0 ? n : max(0, min(n, p + a.right + 1 - j0));
-                    const int from = a.left < 0 ? 0 : max(0, p - a.left - j0), sunk = a.sinks - j0;
+                    const int end = a.right < 0 ? n : min(n, p + a.right + 1 - j0);
+                    const int from = a.left < 0 ? 0 : p - a.left - j0, sunk = a.sinks - j0;
 #pragma unroll
-                    for (int j = 0; j < BK; j++)
-                        if (j >= end || (j < from && j >= sunk)) s[j] = -INFINITY;
+                    for (int c = 0; c < BK / 32; c++) {
+                        const uint32_t seen = below(end - c * 32) & (~below(from - c * 32) | below(sunk - c * 32));
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (!(seen >> x & 1u)) s[c * 32 + x] = -INFINITY;
+                    }
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < BK; j += 8)
+                for (int c = 0; c < BK / 32; c++)
+                    if (c * 32 < n) {
 #pragma unroll
-                    for (int x = 0; x < 4; x++) top[x] = fmaxf(fmaxf(top[x], s[j + x]), s[j + 4 + x]);
+                        for (int x = 0; x < 32; x += 2) top[x / 2 & 3] = max3(top[x / 2 & 3], s[c * 32 + x], s[c * 32 + x + 1]);
+                    }
                 const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
                 // O's row is zero while no key was seen: nothing to rescale then
                 float keep = 1.0f;
@@ -229,34 +302,13 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                     l *= keep;
                     for (int c = 0; c < dn; c += 16) {
                         float o[16];
-                        uint32_t *r = reinterpret_cast<uint32_t *>(o);
-                        asm volatile(
-                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                            : "r"(mine + O_COL + c));
+                        tmem_load16(mine + O_COL + c, o);
                         tmem_wait_load();
 #pragma unroll
                         for (int x = 0; x < 16; x++) o[x] *= keep;
-                        tmem_store16(mine + O_COL + c, r);
+                        tmem_store16(mine + O_COL + c, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < BK / 32; c++) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float e0 = exp2_fast(fmaf(s[c * 32 + 2 * x], a.scale_log2, -base));
-                        const float e1 = exp2_fast(fmaf(s[c * 32 + 2 * x + 1], a.scale_log2, -base));
-                        sum[x & 1] += e0;
-                        sum[2 + (x & 1)] += e1;
-                        w[x] = pack2<T>(e0, e1);
-                    }
-                    tmem_store16(mine + c * 16, w);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 // rows of V past the lane's keys, up to the product's step of 16:
                 // whatever lies there, zero
                 if (n & 15) {
@@ -268,13 +320,32 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                tmem_wait_store();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(p_bar);
+                const float base = m == -INFINITY ? 0.0f : -m;
+                const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(base, base);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int c = 0; c < BK / 32; c++) {
+                    if (c * 32 < n) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            float2 e = ffma2(make_float2(s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]), scale2, base2);
+                            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            sum[x & 1] = fadd2(sum[x & 1], e);
+                            w[x] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_store16(mine + c * 16, w);
+                    }
+                    if (c & 1) {  // half of P: its product may begin
+                        tmem_wait_store();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive(p_bar + (c >> 1) * 8);
+                    }
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             if (tl.n > 0 && ok) ok = wait(o_bar, (tile_turn + tl.n - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
             fence_after();
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bool bad = !ok || !(l < INFINITY);
@@ -282,12 +353,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
             if (ok) {
                 for (int c = 0; c < dn; c += 16) {
                     float o[16];
-                    uint32_t *r = reinterpret_cast<uint32_t *>(o);
-                    asm volatile(
-                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                        : "r"(mine + O_COL + c));
+                    tmem_load16(mine + O_COL + c, o);
                     tmem_wait_load();
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
@@ -326,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     }
     fence_before();
     __syncthreads();
-    if (warp == SOFTMAX_WARPS) {
+    if (warp == MMA_WARP) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
     }
