@@ -2,24 +2,25 @@
 // and bf16, rows and heads on 16-byte borders).
 //
 // A block takes 128 queries of one head (a thread a row) and walks the key
-// tiles they see: the sinks, then up to 128 keys at a time from the window's
+// tiles they see: the sinks, then up to 64 keys at a time from the window's
 // first key on, the last tile in steps of 16. Per tile:
 //     S = Q K^T      tcgen05.mma, Q and K in shared memory (TMA, 128-byte
 //                    swizzle), S in tensor memory
-//     softmax        four warps: a row's 128 scores in registers, P back into
+//     softmax        four warps: a row's 64 scores in registers, P back into
 //                    S's place in 16 bits
 //     O += P V       tcgen05.mma, P from tensor memory, V as it lies in shared
 //                    memory (its head dimension is the instruction's N)
-// One thread issues the products, one the copies. Two blocks share an SM (256 columns
-// of tensor memory and 96 KB of shared memory each), so that one's products
-// run under the other's softmax; inside a block the steps follow one another
-// and nothing needs a second buffer: K is refilled under the softmax, V under
-// the next product.
+// One warp issues the products, one the copies. S, K and V have two buffers, so
+// that the next tile's scores are there when a tile's softmax ends; two
+// blocks share an SM (256 columns of tensor memory and 96 KB of shared memory
+// each) for the rest. Tiles of 128 keys leave no room for a second S beside
+// an O of 128 columns, and were slower though a product of N = 64 costs 48
+// cycles where half of one of N = 128 costs 32.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (the weights stay below 2^8, their sums in f32), which is rare
 // after the first tile. Bound by the exponentials (16 a cycle and SM) and the
-// products (1024 cycles a tile of 128 keys at head size 128) alike.
+// products (1280 cycles a 128 keys at head size 128) alike.
 #include <type_traits>
 
 #include "attn.cuh"
@@ -29,10 +30,10 @@ namespace ppocr {
 
 namespace {
 
-constexpr int BQ = 128, BK = 128, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
+constexpr int BQ = 128, BK = 64, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
 constexpr int BOX = 32;                    // rows a copy brings: 4 KB of one 64-column panel
 constexpr int BOX_BYTES = BOX * 128;
-constexpr int TMEM_COLS = 256;             // S (and P in its place): 0 to 127, O: 128 to 255
+constexpr int TMEM_COLS = 256;             // two S (and P in their places): 0 to 127, O: 128 to 255
 constexpr int O_COL = 128;
 constexpr float GROW = 8.0f;               // log2 of how far a maximum may grow before O is rescaled
 
@@ -147,7 +148,9 @@ struct Tiles {
 template <class T>
 __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ uint64_t bars[7];  // Q, K and V have come; S is done; P's halves are there; O is done
+    // Q has come; then a pair each, used in turn: K and V have come, S is done, P
+    // is there, O is done
+    __shared__ uint64_t bars[11];
     __shared__ uint32_t tmem_s;
     __shared__ int give_up_s;
     // the warp's number and the tensor memory's address by a shuffle, which the
@@ -156,12 +159,13 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     // each operand moved there first)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid & 31;
     const int panels = (a.d + 63) / 64, dn = (a.d + 15) / 16 * 16;  // 64-column panels; head size in steps of 16
-    const uint32_t q_s = shared_u32(smem), k_s = q_s + panels * (BQ * 128), v_s = k_s + panels * (BK * 128);
-    const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 16, s_bar = q_bar + 24, o_bar = q_bar + 32,
-                   p_bar = q_bar + 40;
+    const uint32_t tile_bytes = uint32_t(panels * (BK * 128));      // of one K or V buffer
+    const uint32_t q_s = shared_u32(smem), k_s = q_s + panels * (BQ * 128), v_s = k_s + 2 * tile_bytes;
+    const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 24, s_bar = q_bar + 40, p_bar = q_bar + 56,
+                   o_bar = q_bar + 72;
     volatile int *give_up = &give_up_s;
     if (tid == 0) {
-        for (int i = 0; i < 7; i++) bar_init(q_bar + 8 * i, i >= 5 ? SOFTMAX_WARPS : 1);
+        for (int i = 0; i < 11; i++) bar_init(q_bar + 8 * i, i == 7 || i == 8 ? SOFTMAX_WARPS : 1);
         give_up_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -186,137 +190,146 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     ln.q0 = __shfl_sync(0xffffffffu, ln.q0, 0), ln.k0 = __shfl_sync(0xffffffffu, ln.k0, 0);
     ln.nq = __shfl_sync(0xffffffffu, ln.nq, 0), ln.nk = __shfl_sync(0xffffffffu, ln.nk, 0);
     const int h = blockIdx.y, kvh = h / a.share;
-    uint32_t turn = 0, tile_turn = 0;  // query tiles and key tiles so far: the barriers' phases
-    for (int64_t i0 = int64_t(blockIdx.x) * BQ; i0 < ln.nq; i0 += int64_t(gridDim.x) * BQ, turn++) {
+    // query tiles with keys, and key tiles, so far: tile x uses buffer x % 2 in its phase x / 2 % 2
+    uint32_t turn = 0, done = 0;
+    for (int64_t i0 = int64_t(blockIdx.x) * BQ; i0 < ln.nq; i0 += int64_t(gridDim.x) * BQ) {
         const int rows = int(ln.nq - i0 < BQ ? ln.nq - i0 : BQ);
         const int p0 = int(i0) + ln.nk - ln.nq;
         const Tiles tl(a, p0, p0 + rows - 1, ln.nk);
+        const auto buf = [&](int it) { return (done + uint32_t(it)) & 1u; };
+        const auto phase = [&](int it) { return (done + uint32_t(it)) >> 1 & 1u; };
         if (warp == COPY_WARP) {
             if (tl.n > 0) {
-                const auto load = [&](const CUtensorMap *map, uint32_t to, int head, int64_t row, int n, uint32_t bar) {
+                const auto load = [&](const CUtensorMap *map, uint32_t to, uint32_t panel, int head, int64_t row, int n, uint32_t bar) {
                     const int boxes = (n + BOX - 1) / BOX;
                     if (!one) return;
                     arrive_expect(bar, uint32_t(boxes * panels * BOX_BYTES));
                     for (int p = 0; p < panels; p++)
                         for (int b = 0; b < boxes; b++)
-                            tma_load_3d(to + uint32_t(p * (BK * 128) + b * BOX_BYTES), map, p * 64, head, int(row) + b * BOX, bar);
+                            tma_load_3d(to + p * panel + uint32_t(b * BOX_BYTES), map, p * 64, head, int(row) + b * BOX, bar);
                 };
-                load(&maps.q, q_s, h, ln.q0 + i0, rows, q_bar);
-                load(&maps.k, k_s, kvh, ln.k0 + tl.first(0), tl.count(0), k_bar);
-                load(&maps.v, v_s, kvh, ln.k0 + tl.first(0), tl.count(0), v_bar);
-                for (int it = 1; it < tl.n; it++) {
-                    const uint32_t before = (tile_turn + it - 1) & 1;
-                    if (!wait(s_bar, before)) break;  // K is read
-                    load(&maps.k, k_s, kvh, ln.k0 + tl.first(it), tl.count(it), k_bar);
-                    if (!wait(o_bar, before)) break;  // V is read
-                    load(&maps.v, v_s, kvh, ln.k0 + tl.first(it), tl.count(it), v_bar);
+                const auto load_k = [&](int it) {
+                    load(&maps.k, k_s + buf(it) * tile_bytes, BK * 128, kvh, ln.k0 + tl.first(it), tl.count(it), k_bar + buf(it) * 8);
+                };
+                const auto load_v = [&](int it) {
+                    load(&maps.v, v_s + buf(it) * tile_bytes, BK * 128, kvh, ln.k0 + tl.first(it), tl.count(it), v_bar + buf(it) * 8);
+                };
+                load(&maps.q, q_s, BQ * 128, h, ln.q0 + i0, rows, q_bar);
+                load_k(0);
+                if (tl.n > 1) load_k(1);
+                load_v(0);
+                if (tl.n > 1) load_v(1);
+                for (int it = 2; it < tl.n; it++) {
+                    if (!wait(s_bar + buf(it) * 8, phase(it - 2))) break;  // K is read
+                    load_k(it);
+                    if (!wait(o_bar + buf(it) * 8, phase(it - 2))) break;  // V is read
+                    load_v(it);
                 }
             }
             __syncwarp();
         } else if (warp == MMA_WARP) {
             if (tl.n > 0) {
                 const uint64_t q_desc = desc(q_s, 16, 1024), k_desc = desc(k_s, 16, 1024), v_desc = desc(v_s, BK * 128, 1024);
+                const uint64_t next = tile_bytes / 16;  // the descriptors' addresses count 16 bytes
                 const uint32_t id_o = idesc<T>(dn, 1);
                 const int steps = dn / 16;
-                // no early way out of the loop: its control stays the same in every
-                // lane, and after a wait that ran out no product is issued
+                // The tensor core runs one thread's products in order: S of tile it + 1 goes
+                // ahead of tile it's second product, and takes the place of P two tiles
+                // back behind the product that read it. No early way out of the loop: its
+                // control stays the same in every lane, and after a wait that ran out no
+                // product is issued.
                 bool on = wait(q_bar, turn & 1);
-                for (int it = 0; it < tl.n; it++) {
-                    const uint32_t par = (tile_turn + it) & 1;
-                    const int n = (tl.count(it) + 15) / 16;
-                    on &= wait(k_bar, par);
+                const auto scores = [&](int it) {
+                    on &= wait(k_bar + buf(it) * 8, phase(it));
                     fence_after();
-                    const uint32_t id_s = idesc<T>(n * 16, 0);
-                    const uint32_t go = one && on;
+                    const uint32_t id_s = idesc<T>((tl.count(it) + 15) / 16 * 16, 0), go = one && on;
+                    const uint64_t k_at = k_desc + buf(it) * next;
 #pragma unroll
                     for (int kk = 0; kk < 8; kk++) {
-                        // the descriptors' addresses count 16 bytes
-                        constexpr uint64_t panel = BK * 128 / 16;
-                        const uint64_t at = (kk >> 2) * panel + (kk & 3) * 2;
-                        mma_ss(tmem, q_desc + at, k_desc + at, id_s, kk > 0, go & uint32_t(kk < steps));
+                        const uint64_t q_in = (kk >> 2) * (BQ * 128 / 16) + (kk & 3) * 2, k_in = (kk >> 2) * (BK * 128 / 16) + (kk & 3) * 2;
+                        mma_ss(tmem + buf(it) * BK, q_desc + q_in, k_at + k_in, id_s, kk > 0, go & uint32_t(kk < steps));
                     }
-                    commit(s_bar, go);
-                    on &= wait(v_bar, par) && wait(p_bar, par);
+                    commit(s_bar + buf(it) * 8, go);
+                };
+                scores(0);
+                for (int it = 0; it < tl.n; it++) {
+                    if (it + 1 < tl.n) scores(it + 1);
+                    const int n = (tl.count(it) + 15) / 16;
+                    on &= wait(v_bar + buf(it) * 8, phase(it)) && wait(p_bar + buf(it) * 8, phase(it));
                     fence_after();
-                    const uint32_t go1 = one && on;
+                    const uint32_t go = one && on;
+                    const uint64_t v_at = v_desc + buf(it) * next;
 #pragma unroll
-                    for (int kk = 0; kk < BK / 32; kk++)
-                        mma_ts(tmem + O_COL, tmem + kk * 8, v_desc + uint64_t(kk * 128), id_o, it > 0 || kk > 0, go1 & uint32_t(kk < n));
-                    on &= wait(p_bar + 8, par);
-                    fence_after();
-                    const uint32_t go2 = one && on;
-#pragma unroll
-                    for (int kk = BK / 32; kk < BK / 16; kk++)
-                        mma_ts(tmem + O_COL, tmem + kk * 8, v_desc + uint64_t(kk * 128), id_o, 1, go2 & uint32_t(kk < n));
-                    commit(o_bar, go2);
-                    on &= wait(o_bar, par);  // S's place is free
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        mma_ts(tmem + O_COL, tmem + buf(it) * BK + kk * 8, v_at + uint64_t(kk * 128), id_o, it > 0 || kk > 0,
+                               go & uint32_t(kk < n));
+                    commit(o_bar + buf(it) * 8, go);
                 }
             }
             __syncwarp();
         } else {
             const int row = warp * 32 + lane, p = p0 + row;
-            const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
+            const uint32_t mine = tmem + (uint32_t(warp * 32) << 16), o_at = mine + O_COL;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int it = 0; it < tl.n; it++) {
-                const uint32_t par = (tile_turn + it) & 1;
+                const uint32_t s_at = mine + buf(it) * BK;
                 const int j0 = tl.first(it), n = tl.count(it);
-                ok = wait(s_bar, par);
+                ok = wait(s_bar + buf(it) * 8, phase(it));
                 if (!ok) break;
                 fence_after();
                 float s[BK];
-#pragma unroll
-                for (int c = 0; c < BK / 32; c++)
-                    if (c * 32 < n) tmem_load32(mine + c * 32, s + c * 32);
+                tmem_load32(s_at, s);
+                if (n > 32) tmem_load32(s_at + 32, s + 32);
                 tmem_wait_load();
-                // this row's keys of the tile: a run, and below the sinks' end all
-                // that the right side leaves
-                const bool whole = n % 32 == 0 && (a.right < 0 || j0 + n - 1 <= p0 + warp * 32 + a.right) &&
-                                   (a.left < 0 || j0 >= p0 + warp * 32 + 31 - a.left || j0 + n <= a.sinks);
-                if (!whole) {
-                    const int end = a.right < 0 ? n : min(n, p + a.right + 1 - j0);
-                    const int from = a.left < 0 ? 0 : p - a.left - j0, sunk = a.sinks - j0;
-#pragma unroll
-                    for (int c = 0; c < BK / 32; c++) {
-                        const uint32_t seen = below(end - c * 32) & (~below(from - c * 32) | below(sunk - c * 32));
-#pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (!(seen >> x & 1u)) s[c * 32 + x] = -INFINITY;
-                    }
-                }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < BK / 32; c++)
                     if (c * 32 < n) {
+                        // this row's keys of these 32: a run, and below the sinks' end all that
+                        // the right side leaves
+                        const int j = j0 + c * 32, left = n - c * 32, first = p0 + warp * 32;
+                        const bool whole = left >= 32 && (a.right < 0 || j + 31 <= first + a.right) &&
+                                           (a.left < 0 || j >= first + 31 - a.left || j + 32 <= a.sinks);
+                        if (!whole) {
+                            const uint32_t seen = below(a.right < 0 ? left : min(left, p + a.right + 1 - j)) &
+                                                  (a.left < 0 ? ~0u : ~below(p - a.left - j) | below(a.sinks - j));
+#pragma unroll
+                            for (int x = 0; x < 32; x++)
+                                if (!(seen >> x & 1u)) s[c * 32 + x] = -INFINITY;
+                        }
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) top[x / 2 & 3] = max3(top[x / 2 & 3], s[c * 32 + x], s[c * 32 + x + 1]);
                     }
                 const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
                 // O's row is zero while no key was seen: nothing to rescale then
                 float keep = 1.0f;
-                if (now > m + GROW || m == -INFINITY) {
+                if (now > m + GROW) {
                     keep = m == -INFINITY ? 1.0f : exp2_fast(m - now);
                     m = now;
                 }
                 if (__any_sync(0xffffffffu, keep != 1.0f)) {
+                    ok = wait(o_bar + buf(it + 1) * 8, phase(it - 1));  // the product before is in O
+                    fence_after();
                     l *= keep;
                     for (int c = 0; c < dn; c += 16) {
                         float o[16];
-                        tmem_load16(mine + O_COL + c, o);
+                        tmem_load16(o_at + c, o);
                         tmem_wait_load();
 #pragma unroll
                         for (int x = 0; x < 16; x++) o[x] *= keep;
-                        tmem_store16(mine + O_COL + c, reinterpret_cast<const uint32_t *>(o));
+                        tmem_store16(o_at + c, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
                 // rows of V past the lane's keys, up to the product's step of 16:
                 // whatever lies there, zero
                 if (n & 15) {
-                    ok = wait(v_bar, par);
+                    ok = wait(v_bar + buf(it) * 8, phase(it));
+                    unsigned char *v = smem + (v_s - q_s) + buf(it) * tile_bytes;
                     const int gap = 16 - (n & 15);
                     for (int e = row; e < gap * panels * 8; e += SOFTMAX_WARPS * 32) {
                         const int r = n + e / (panels * 8), c = e % (panels * 8);
-                        *reinterpret_cast<uint4 *>(smem + (v_s - q_s) + (c >> 3) * (BK * 128) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(v + (c >> 3) * (BK * 128) + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
@@ -324,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(base, base);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < BK / 32; c++) {
+                for (int c = 0; c < BK / 32; c++)
                     if (c * 32 < n) {
                         uint32_t w[16];
 #pragma unroll
@@ -334,18 +347,15 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                             sum[x & 1] = fadd2(sum[x & 1], e);
                             w[x] = pack2<T>(e.x, e.y);
                         }
-                        tmem_store16(mine + c * 16, w);
+                        tmem_store16(s_at + c * 16, w);
                     }
-                    if (c & 1) {  // half of P: its product may begin
-                        tmem_wait_store();
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) arrive(p_bar + (c >> 1) * 8);
-                    }
-                }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_wait_store();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(p_bar + buf(it) * 8);
             }
-            if (tl.n > 0 && ok) ok = wait(o_bar, (tile_turn + tl.n - 1) & 1);
+            if (tl.n > 0 && ok) ok = wait(o_bar + buf(tl.n - 1) * 8, phase(tl.n - 1));
             fence_after();
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bool bad = !ok || !(l < INFINITY);
@@ -353,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
             if (ok) {
                 for (int c = 0; c < dn; c += 16) {
                     float o[16];
-                    tmem_load16(mine + O_COL + c, o);
+                    tmem_load16(o_at + c, o);
                     tmem_wait_load();
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
@@ -384,8 +394,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
             }
             fence_before();
         }
-        tile_turn += tl.n;
-        if (tl.n == 0) turn--;
+        done += tl.n;
+        turn += tl.n > 0;
         __syncthreads();  // O is read: the next query tile's product may overwrite it
         fence_after();
         if (*give_up) break;
@@ -412,8 +422,8 @@ bool map_rows(CUtensorMap *map, const void *p, int type, int64_t rows, int64_t r
 
 template <class T>
 cudaError_t start(const AttnArgs &a, const Maps &maps, uint32_t max_q, cudaStream_t stream) {
-    const int panels = (a.d + 63) / 64, shared = 3 * panels * BK * 128;
-    const cudaError_t e = raise_shared<attn_tc_kernel<T>>(3 * 2 * BK * 128);
+    const int panels = (a.d + 63) / 64, shared = panels * 128 * (BQ + 4 * BK);
+    const cudaError_t e = raise_shared<attn_tc_kernel<T>>(2 * 128 * (BQ + 4 * BK));
     if (e != cudaSuccess) return e;
     const uint32_t tiles = max_q ? (max_q + BQ - 1) / BQ : 1;
     attn_tc_kernel<T><<<dim3(tiles, unsigned(a.heads), unsigned(a.lanes)), THREADS, shared, stream>>>(a, maps);
