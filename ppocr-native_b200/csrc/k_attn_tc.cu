@@ -126,6 +126,31 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// The slow half of a wait; a lane that was told to give up says so to all.
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile int *give_up) {
+    if (*give_up) return false;
+    if (wait_copy(bar, parity)) return true;
+    *give_up = 1;
+    return false;
+}
+
+// 2^x for x up to 16 on the multiply-add pipe, two at a time: x = n + f with f in
+// [-1/2, 1/2], 2^f by a polynomial of degree 4 (minimax by Lawson's weights,
+// 2.6e-6 relative), n into the exponent. Below -125: 2^-125.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+    const float round = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers, which its low bits then hold
+    const float2 r = fadd2(x, make_float2(round, round));
+    const float2 f = ffma2(fadd2(r, make_float2(-round, -round)), make_float2(-1.0f, -1.0f), x);
+    const auto both = [](float c) { return make_float2(c, c); };
+    float2 p = ffma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+    p = ffma2(p, f, both(0.240247443318367f));
+    p = ffma2(p, f, both(0.6931217908859253f));
+    p = ffma2(p, f, both(0.9999992847442627f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+
 // Bits 0 to n - 1.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
@@ -180,10 +205,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     const bool one = elect_one();
     // a wait that ran out of time ends every role's; the rows are done again the plain way
     const auto wait = [&](uint32_t bar, uint32_t parity) {
-        const bool came = !*give_up && wait_copy(bar, parity);
-        if (__all_sync(0xffffffffu, came)) return true;
-        *give_up = 1;
-        return false;
+        return try_wait(bar, parity) || wait_long(bar, parity, give_up);
     };
 
     Lane ln = read_lane(a, blockIdx.z);
@@ -220,9 +242,9 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 load_v(0);
                 if (tl.n > 1) load_v(1);
                 for (int it = 2; it < tl.n; it++) {
-                    if (!wait(s_bar + buf(it) * 8, phase(it - 2))) break;  // K is read
+                    if (!__all_sync(0xffffffffu, wait(s_bar + buf(it) * 8, phase(it - 2)))) break;  // K is read
                     load_k(it);
-                    if (!wait(o_bar + buf(it) * 8, phase(it - 2))) break;  // V is read
+                    if (!__all_sync(0xffffffffu, wait(o_bar + buf(it) * 8, phase(it - 2)))) break;  // V is read
                     load_v(it);
                 }
             }
@@ -238,9 +260,9 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 // back behind the product that read it. No early way out of the loop: its
                 // control stays the same in every lane, and after a wait that ran out no
                 // product is issued.
-                bool on = wait(q_bar, turn & 1);
+                bool on = __all_sync(0xffffffffu, wait(q_bar, turn & 1));
                 const auto scores = [&](int it) {
-                    on &= wait(k_bar + buf(it) * 8, phase(it));
+                    on &= __all_sync(0xffffffffu, wait(k_bar + buf(it) * 8, phase(it)));
                     fence_after();
                     const uint32_t id_s = idesc<T>((tl.count(it) + 15) / 16 * 16, 0), go = one && on;
                     const uint64_t k_at = k_desc + buf(it) * next;
@@ -255,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 for (int it = 0; it < tl.n; it++) {
                     if (it + 1 < tl.n) scores(it + 1);
                     const int n = (tl.count(it) + 15) / 16;
-                    on &= wait(v_bar + buf(it) * 8, phase(it)) && wait(p_bar + buf(it) * 8, phase(it));
+                    on &= __all_sync(0xffffffffu, wait(v_bar + buf(it) * 8, phase(it)) && wait(p_bar + buf(it) * 8, phase(it)));
                     fence_after();
                     const uint32_t go = one && on;
                     const uint64_t v_at = v_desc + buf(it) * next;
@@ -271,60 +293,68 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
             const int row = warp * 32 + lane, p = p0 + row;
             const uint32_t mine = tmem + (uint32_t(warp * 32) << 16), o_at = mine + O_COL;
             float m = -INFINITY, l = 0.0f;
-            bool ok = true;
+            bool ok = true;  // a wait that ran out spoils the rows, not the warp's common way
+            // the tiles that every row of this block sees whole
+            const int whole_from = tl.n_sink + (a.left < 0 ? 0 : max(0, p0 + BQ - 1 - a.left - tl.lo + BK - 1) / BK);
+            const int whole_to = tl.n_sink + (min(tl.hi, a.right < 0 ? tl.hi : p0 + a.right + 1) - tl.lo) / BK;
             for (int it = 0; it < tl.n; it++) {
                 const uint32_t s_at = mine + buf(it) * BK;
                 const int j0 = tl.first(it), n = tl.count(it);
-                ok = wait(s_bar + buf(it) * 8, phase(it));
-                if (!ok) break;
+                ok &= wait(s_bar + buf(it) * 8, phase(it));
                 fence_after();
                 float s[BK];
                 tmem_load32(s_at, s);
                 if (n > 32) tmem_load32(s_at + 32, s + 32);
                 tmem_wait_load();
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (it < whole_from || it >= whole_to) {
+#pragma unroll
+                    for (int c = 0; c < BK / 32; c++) {
+                        // this row's keys of these 32: a run, and below the sinks' end all that
+                        // the right side leaves
+                        const int j = j0 + c * 32, left = n - c * 32;
+                        const uint32_t seen = below(a.right < 0 ? left : min(left, p + a.right + 1 - j)) &
+                                              (a.left < 0 ? ~0u : ~below(p - a.left - j) | below(a.sinks - j));
+                        if (__all_sync(0xffffffffu, seen == ~0u)) continue;
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (!(seen >> x & 1u)) s[c * 32 + x] = -INFINITY;
+                    }
+                }
 #pragma unroll
                 for (int c = 0; c < BK / 32; c++)
                     if (c * 32 < n) {
-                        // this row's keys of these 32: a run, and below the sinks' end all that
-                        // the right side leaves
-                        const int j = j0 + c * 32, left = n - c * 32, first = p0 + warp * 32;
-                        const bool whole = left >= 32 && (a.right < 0 || j + 31 <= first + a.right) &&
-                                           (a.left < 0 || j >= first + 31 - a.left || j + 32 <= a.sinks);
-                        if (!whole) {
-                            const uint32_t seen = below(a.right < 0 ? left : min(left, p + a.right + 1 - j)) &
-                                                  (a.left < 0 ? ~0u : ~below(p - a.left - j) | below(a.sinks - j));
-#pragma unroll
-                            for (int x = 0; x < 32; x++)
-                                if (!(seen >> x & 1u)) s[c * 32 + x] = -INFINITY;
-                        }
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) top[x / 2 & 3] = max3(top[x / 2 & 3], s[c * 32 + x], s[c * 32 + x + 1]);
                     }
                 const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-                // O's row is zero while no key was seen: nothing to rescale then
-                float keep = 1.0f;
-                if (now > m + GROW) {
-                    keep = m == -INFINITY ? 1.0f : exp2_fast(m - now);
-                    m = now;
-                }
-                if (__any_sync(0xffffffffu, keep != 1.0f)) {
-                    ok = wait(o_bar + buf(it + 1) * 8, phase(it - 1));  // the product before is in O
-                    fence_after();
-                    l *= keep;
-                    for (int c = 0; c < dn; c += 16) {
-                        float o[16];
-                        tmem_load16(o_at + c, o);
-                        tmem_wait_load();
+                const bool grown = now > m + GROW;
+                if (__any_sync(0xffffffffu, grown)) {
+                    // O's row is zero while no key was seen: nothing to rescale then
+                    float keep = 1.0f;
+                    if (grown) {
+                        keep = m == -INFINITY ? 1.0f : exp2_fast(m - now);
+                        m = now;
+                    }
+                    if (__any_sync(0xffffffffu, keep != 1.0f)) {
+                        ok &= wait(o_bar + buf(it + 1) * 8, phase(it - 1));  // the product before is in O
+                        fence_after();
+                        __syncwarp();
+                        l *= keep;
+                        for (int c = 0; c < dn; c += 16) {
+                            float o[16];
+                            tmem_load16(o_at + c, o);
+                            tmem_wait_load();
 #pragma unroll
-                        for (int x = 0; x < 16; x++) o[x] *= keep;
-                        tmem_store16(o_at + c, reinterpret_cast<const uint32_t *>(o));
+                            for (int x = 0; x < 16; x++) o[x] *= keep;
+                            tmem_store16(o_at + c, reinterpret_cast<const uint32_t *>(o));
+                        }
                     }
                 }
                 // rows of V past the lane's keys, up to the product's step of 16:
                 // whatever lies there, zero
                 if (n & 15) {
-                    ok = wait(v_bar + buf(it) * 8, phase(it));
+                    ok &= wait(v_bar + buf(it) * 8, phase(it));
                     unsigned char *v = smem + (v_s - q_s) + buf(it) * tile_bytes;
                     const int gap = 16 - (n & 15);
                     for (int e = row; e < gap * panels * 8; e += SOFTMAX_WARPS * 32) {
@@ -343,7 +373,8 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
                             float2 e = ffma2(make_float2(s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]), scale2, base2);
-                            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            // a quarter of the exponentials beside the special-function unit
+                            e = x % 4 == 3 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
                             sum[x & 1] = fadd2(sum[x & 1], e);
                             w[x] = pack2<T>(e.x, e.y);
                         }
@@ -355,8 +386,10 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
                 __syncwarp();
                 if (lane == 0) arrive(p_bar + buf(it) * 8);
             }
-            if (tl.n > 0 && ok) ok = wait(o_bar + buf(tl.n - 1) * 8, phase(tl.n - 1));
+            if (tl.n > 0) ok &= wait(o_bar + buf(tl.n - 1) * 8, phase(tl.n - 1));
+            ok = __all_sync(0xffffffffu, ok);
             fence_after();
+            if (m == -INFINITY) l = 0.0f;  // no key was seen (the polynomial makes 2^-125 of a hidden one)
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bool bad = !ok || !(l < INFINITY);
             T *out = static_cast<T *>(a.out) + (ln.q0 + i0 + row) * a.out_row + h * a.out_head;
