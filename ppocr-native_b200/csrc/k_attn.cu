@@ -4,9 +4,11 @@
 //
 // A block of four warps takes 64 queries of one head, 16 a warp, and walks
 // the key tiles they see (sinks, then the window), 64 keys a tile, two
-// buffers filled by cp.async while the other is used; tiles outside every
-// query's window are never read, tiles inside every window skip the masks.
-// Bound by the warp-level matrix instructions.
+// buffers filled by cp.async while the other is used (32 in f32, whose
+// products are three each: a finer step leaves less of a narrow window's tiles
+// hidden); tiles outside every query's window are never read, those outside a
+// warp's are skipped, tiles inside every window skip the masks. Bound by the
+// warp-level matrix instructions.
 #include <cmath>
 
 #include "attn.cuh"
@@ -19,7 +21,7 @@ constexpr int BQ = 64, ROW_THREADS = 128;
 
 template <class T, int DP>
 struct RowTile {
-    static constexpr int BK = sizeof(T) == 4 && DP > 64 ? 32 : 64;
+    static constexpr int BK = sizeof(T) == 4 ? 32 : 64;
     static constexpr int STRIDE = TileOf<T, DP>::STRIDE;
     static constexpr int Q_BYTES = BQ * STRIDE * int(sizeof(T)), K_BYTES = BK * STRIDE * int(sizeof(T));
     static constexpr int SHARED = Q_BYTES + 4 * K_BYTES;
@@ -67,6 +69,8 @@ __global__ void __launch_bounds__(ROW_THREADS) attn_rows_kernel(const __grid_con
             copy_commit();
             const uint32_t ks = kv + (it & 1) * 2 * R::K_BYTES, vs = ks + R::K_BYTES;
             const int j0 = kt.first<BK>(it), jend = kt.end(it);
+            // nothing here for this warp's rows
+            if ((a.right >= 0 && j0 > pw + 15 + a.right) || (a.left >= 0 && jend <= pw - a.left && j0 >= a.sinks)) continue;
             float s[BK / 8][4];
             w.template scores<BK / 8>(s, qw, ks, lane);
             const bool whole = j0 + BK <= jend && (a.right < 0 || j0 + BK - 1 <= pw + a.right) &&

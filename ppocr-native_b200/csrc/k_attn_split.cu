@@ -4,9 +4,10 @@
 // Rows of a tile are the queries that read one key head (query i, head h of
 // its group), up to 16. A cluster of up to eight blocks takes one tile; its
 // 4 * blocks warps take the key tiles in turn, each with a ring of its own
-// filled by cp.async and a softmax state of its own (m, l, o). The states
-// meet through distributed shared memory: row r is joined by block r mod
-// cluster, with weights 2^(m_i - max m). No workspace, nothing to clear.
+// filled by cp.async and a softmax state of its own (m, l, o). A block's four
+// states become one in its shared memory, with weights 2^(m_i - max m), and the
+// cluster's meet through distributed shared memory: row r is joined by block
+// r mod cluster. No workspace, nothing to clear.
 // Bound by the keys' and values' bytes; a single lane by latency.
 #include "attn.cuh"
 
@@ -14,7 +15,7 @@ namespace ppocr {
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3;
+constexpr int WARPS = 4, THREADS = WARPS * 32, STAGES = 3, MOST_BLOCKS = 8;
 
 template <class T, int DP>
 struct SplitTile {
@@ -24,7 +25,8 @@ struct SplitTile {
     static constexpr int RING = STAGES * 2 * K_BYTES;  // one warp's
     // a warp's joined state reuses its ring: o[16][DP], m[16], l[16]
     static_assert(RING >= (16 * DP + 32) * 4, "the state fits the ring");
-    static constexpr int SHARED = Q_BYTES + WARPS * RING;
+    static constexpr int JOIN = (16 * DP + 32) * 4;  // the block's joined state
+    static constexpr int SHARED = Q_BYTES + WARPS * RING + JOIN;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -50,6 +52,19 @@ __device__ __forceinline__ float peer_load(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ float lds(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts2(uint32_t addr, float x, float y) {
+    asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
+}
 __device__ __forceinline__ void sts(uint32_t addr, float v) {
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
@@ -60,7 +75,7 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
     constexpr int BK = R::BK, STRIDE = R::STRIDE;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const uint32_t qs = shared_u32(smem), rings = qs + R::Q_BYTES, ring = rings + warp * R::RING;
+    const uint32_t qs = shared_u32(smem), rings = qs + R::Q_BYTES, ring = rings + warp * R::RING, joined = rings + WARPS * R::RING;
     const int blocks = int(cluster_size()), rank = int(cluster_rank()), workers = blocks * WARPS;
     const Lane ln = read_lane(a, blockIdx.z);
     const int kvh = blockIdx.y;
@@ -130,46 +145,79 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
             w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 1);
             w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 2);
             const int row = (lane >> 2) + 8 * r;
+            if (row >= rows) continue;
             if ((lane & 3) == 0) {
                 sts(ring + uint32_t((16 * DP + row) * 4), w.m[r]);
                 sts(ring + uint32_t((16 * DP + 16 + row) * 4), w.l[r]);
             }
 #pragma unroll
-            for (int n = 0; n < DP / 8; n++) {
-                sts(ring + uint32_t((row * DP + n * 8 + (lane & 3) * 2) * 4), w.o[n][2 * r]);
-                sts(ring + uint32_t((row * DP + n * 8 + (lane & 3) * 2 + 1) * 4), w.o[n][2 * r + 1]);
+            for (int n = 0; n < DP / 8; n++)
+                sts2(ring + uint32_t((row * DP + n * 8 + (lane & 3) * 2) * 4), w.o[n][2 * r], w.o[n][2 * r + 1]);
+        }
+        __syncthreads();
+        // the block's four states as one, a quarter of a warp's lanes' values
+        // (4 columns) a thread
+        constexpr int Q4 = DP / 4;
+        for (int e = tid; e < rows * Q4; e += THREADS) {
+            const int r = e / Q4, c = e % Q4 * 4;
+            float m[WARPS], top = -INFINITY, sum = 0.0f;
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int x = 0; x < WARPS; x++) {
+                m[x] = lds(rings + uint32_t(x * R::RING + (16 * DP + r) * 4));
+                top = fmaxf(top, m[x]);
+            }
+#pragma unroll
+            for (int x = 0; x < WARPS; x++) {
+                const float f = exp2_fast(m[x] - (top == -INFINITY ? 0.0f : top));
+                const float4 o = lds4(rings + uint32_t(x * R::RING + (r * DP + c) * 4));
+                sum = fmaf(f, lds(rings + uint32_t(x * R::RING + (16 * DP + 16 + r) * 4)), sum);
+                acc = make_float4(fmaf(f, o.x, acc.x), fmaf(f, o.y, acc.y), fmaf(f, o.z, acc.z), fmaf(f, o.w, acc.w));
+            }
+            sts2(joined + uint32_t((r * DP + c) * 4), acc.x, acc.y);
+            sts2(joined + uint32_t((r * DP + c + 2) * 4), acc.z, acc.w);
+            if (c == 0) {
+                sts(joined + uint32_t((16 * DP + r) * 4), top);
+                sts(joined + uint32_t((16 * DP + 16 + r) * 4), sum);
             }
         }
-        cluster_sync();
+        if (blocks > 1)
+            cluster_sync();
+        else
+            __syncthreads();
 
+        // then the cluster's: row r by block r mod blocks, a warp a row
         for (int r = rank + warp * blocks; r < rows; r += workers) {
-            // lane x holds worker x's maximum and sum (at most 32 workers)
-            float m = -INFINITY, l = 0.0f;
-            if (lane < workers) {
-                const uint32_t at = peer_addr(rings + uint32_t((lane % WARPS) * R::RING), uint32_t(lane / WARPS));
-                m = peer_load(at + uint32_t((16 * DP + r) * 4));
-                l = peer_load(at + uint32_t((16 * DP + 16 + r) * 4));
+            float m[MOST_BLOCKS], top = -INFINITY, sum = 0.0f;
+            uint32_t from[MOST_BLOCKS];
+#pragma unroll
+            for (int x = 0; x < MOST_BLOCKS; x++) {
+                from[x] = x < blocks ? peer_addr(joined, uint32_t(x)) : 0;
+                m[x] = x < blocks ? peer_load(from[x] + uint32_t((16 * DP + r) * 4)) : -INFINITY;
             }
-            float top = m;
+            float part[MOST_BLOCKS];
 #pragma unroll
-            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float share = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
-            float sum = l * share;
-#pragma unroll
-            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            float acc[(DP + 31) / 32] = {};
-#pragma unroll 4
-            for (int x = 0; x < workers; x++) {
-                const float c = __shfl_sync(0xffffffffu, share, x);
-                const uint32_t at = peer_addr(rings + uint32_t((x % WARPS) * R::RING), uint32_t(x / WARPS));
-#pragma unroll
-                for (int e = 0; e < (DP + 31) / 32; e++)
-                    if (lane + 32 * e < DP) acc[e] = fmaf(c, peer_load(at + uint32_t((r * DP + lane + 32 * e) * 4)), acc[e]);
+            for (int x = 0; x < MOST_BLOCKS; x++) {
+                part[x] = x < blocks ? peer_load(from[x] + uint32_t((16 * DP + 16 + r) * 4)) : 0.0f;
+                top = fmaxf(top, m[x]);
             }
+#pragma unroll
+            for (int x = 0; x < MOST_BLOCKS; x++) {
+                m[x] = exp2_fast(m[x] - (top == -INFINITY ? 0.0f : top));
+                sum = fmaf(m[x], part[x], sum);
+            }
+            constexpr int E = (DP + 31) / 32;
+            float acc[E] = {};
+#pragma unroll
+            for (int x = 0; x < MOST_BLOCKS; x++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (x < blocks && lane + 32 * e < DP)
+                        acc[e] = fmaf(m[x], peer_load(from[x] + uint32_t((r * DP + lane + 32 * e) * 4)), acc[e]);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             bool bad = false;
 #pragma unroll
-            for (int e = 0; e < (DP + 31) / 32; e++) {
+            for (int e = 0; e < E; e++) {
                 acc[e] *= inv;
                 bad |= !(fabsf(acc[e]) < INFINITY);
             }
@@ -179,11 +227,14 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
             } else {
                 T *out = static_cast<T *>(a.out) + (ln.q0 + i) * a.out_row + h * a.out_head;
 #pragma unroll
-                for (int e = 0; e < (DP + 31) / 32; e++)
+                for (int e = 0; e < E; e++)
                     if (lane + 32 * e < a.d) out[lane + 32 * e] = from_f32<T>(acc[e]);
             }
         }
-        cluster_sync();  // no block overwrites or leaves what another still reads
+        if (blocks > 1)
+            cluster_sync();  // no block overwrites or leaves what another still reads
+        else
+            __syncthreads();
     }
 }
 
@@ -196,7 +247,7 @@ cudaError_t start_split(const AttnArgs &a, uint32_t max_q, uint32_t max_keys, cu
     const uint64_t alone = tiles * a.lanes * a.kv_heads;
     // blocks a tile: until the card is full or every warp has one key tile
     uint32_t blocks = 1;
-    while (blocks < 8 && alone * blocks < uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
+    while (blocks < MOST_BLOCKS && alone * blocks < uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(unsigned(tiles * blocks), unsigned(a.kv_heads), unsigned(a.lanes));
     c.blockDim = dim3(THREADS);

@@ -189,6 +189,16 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     const uint32_t q_bar = shared_u32(bars), k_bar = q_bar + 8, v_bar = q_bar + 24, s_bar = q_bar + 40, p_bar = q_bar + 56,
                    o_bar = q_bar + 72;
     volatile int *give_up = &give_up_s;
+    // the lane first: most blocks of a ragged batch's grid have no queries
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
+    Lane ln = read_lane(a, blockIdx.z);
+    ln.q0 = __shfl_sync(0xffffffffu, ln.q0, 0), ln.k0 = __shfl_sync(0xffffffffu, ln.k0, 0);
+    ln.nq = __shfl_sync(0xffffffffu, ln.nq, 0), ln.nk = __shfl_sync(0xffffffffu, ln.nk, 0);
+    if (int64_t(blockIdx.x) * BQ >= ln.nq) return;
     if (tid == 0) {
         for (int i = 0; i < 11; i++) bar_init(q_bar + 8 * i, i == 7 || i == 8 ? SOFTMAX_WARPS : 1);
         give_up_s = 0;
@@ -208,9 +218,6 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
         return try_wait(bar, parity) || wait_long(bar, parity, give_up);
     };
 
-    Lane ln = read_lane(a, blockIdx.z);
-    ln.q0 = __shfl_sync(0xffffffffu, ln.q0, 0), ln.k0 = __shfl_sync(0xffffffffu, ln.k0, 0);
-    ln.nq = __shfl_sync(0xffffffffu, ln.nq, 0), ln.nk = __shfl_sync(0xffffffffu, ln.nk, 0);
     const int h = blockIdx.y, kvh = h / a.share;
     // query tiles with keys, and key tiles, so far: tile x uses buffer x % 2 in its phase x / 2 % 2
     uint32_t turn = 0, done = 0;
