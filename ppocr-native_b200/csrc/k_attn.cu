@@ -22,13 +22,14 @@ constexpr int BQ = 64, ROW_THREADS = 128;
 template <class T, int DP>
 struct RowTile {
     static constexpr int BK = sizeof(T) == 4 ? 32 : 64;
+    static constexpr int BLOCKS = DP <= 32 ? 5 : DP <= 64 ? 3 : 2;  // an SM, by registers
     static constexpr int STRIDE = TileOf<T, DP>::STRIDE;
     static constexpr int Q_BYTES = BQ * STRIDE * int(sizeof(T)), K_BYTES = BK * STRIDE * int(sizeof(T));
     static constexpr int SHARED = Q_BYTES + 4 * K_BYTES;
 };
 
 template <class T, int DP>
-__global__ void __launch_bounds__(ROW_THREADS) attn_rows_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(ROW_THREADS, RowTile<T, DP>::BLOCKS) attn_rows_kernel(const __grid_constant__ AttnArgs a) {
     using R = RowTile<T, DP>;
     constexpr int BK = R::BK, STRIDE = R::STRIDE;
     extern __shared__ __align__(16) unsigned char smem[];

@@ -30,11 +30,9 @@ namespace ppocr {
 
 namespace {
 
-constexpr int BQ = 128, BK = 64, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
+constexpr int BQ = 128, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
 constexpr int BOX = 32;                    // rows a copy brings: 4 KB of one 64-column panel
 constexpr int BOX_BYTES = BOX * 128;
-constexpr int TMEM_COLS = 256;             // two S (and P in their places): 0 to 127, O: 128 to 255
-constexpr int O_COL = 128;
 constexpr float GROW = 8.0f;               // log2 of how far a maximum may grow before O is rescaled
 
 struct Maps {
@@ -155,6 +153,7 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 // The tiles of one query tile: the sinks below the window, then the window.
+template <int BK>
 struct Tiles {
     int sink_end, lo, hi, n_sink, n;
     __device__ __forceinline__ Tiles(const AttnArgs &a, int p0, int p1, int nk) {
@@ -170,8 +169,12 @@ struct Tiles {
     }
 };
 
-template <class T>
-__global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
+// BK keys a tile. Head sizes above 64: 64 keys, 256 columns of tensor memory (two
+// S and P in their places, then 128 of O), two blocks an SM; up to 64: 32 keys,
+// 128 columns (O has 64), four.
+template <class T, int BK>
+__global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ Maps maps) {
+    constexpr int O_COL = 2 * BK, TMEM_COLS = BK == 64 ? 256 : 128;
     extern __shared__ __align__(1024) unsigned char smem[];
     // Q has come; then a pair each, used in turn: K and V have come, S is done, P
     // is there, O is done
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 2) attn_tc_kernel(const __grid_consta
     for (int64_t i0 = int64_t(blockIdx.x) * BQ; i0 < ln.nq; i0 += int64_t(gridDim.x) * BQ) {
         const int rows = int(ln.nq - i0 < BQ ? ln.nq - i0 : BQ);
         const int p0 = int(i0) + ln.nk - ln.nq;
-        const Tiles tl(a, p0, p0 + rows - 1, ln.nk);
+        const Tiles<BK> tl(a, p0, p0 + rows - 1, ln.nk);
         const auto buf = [&](int it) { return (done + uint32_t(it)) & 1u; };
         const auto phase = [&](int it) { return (done + uint32_t(it)) >> 1 & 1u; };
         if (warp == COPY_WARP) {
@@ -460,14 +463,19 @@ bool map_rows(CUtensorMap *map, const void *p, int type, int64_t rows, int64_t r
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T>
+template <class T, int BK>
 cudaError_t start(const AttnArgs &a, const Maps &maps, uint32_t max_q, cudaStream_t stream) {
     const int panels = (a.d + 63) / 64, shared = panels * 128 * (BQ + 4 * BK);
-    const cudaError_t e = raise_shared<attn_tc_kernel<T>>(2 * 128 * (BQ + 4 * BK));
+    const cudaError_t e = raise_shared<attn_tc_kernel<T, BK>>((BK == 64 ? 2 : 1) * 128 * (BQ + 4 * BK));
     if (e != cudaSuccess) return e;
     const uint32_t tiles = max_q ? (max_q + BQ - 1) / BQ : 1;
-    attn_tc_kernel<T><<<dim3(tiles, unsigned(a.heads), unsigned(a.lanes)), THREADS, shared, stream>>>(a, maps);
+    attn_tc_kernel<T, BK><<<dim3(tiles, unsigned(a.heads), unsigned(a.lanes)), THREADS, shared, stream>>>(a, maps);
     return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t start_d(const AttnArgs &a, const Maps &maps, uint32_t max_q, cudaStream_t stream) {
+    return a.d > 64 ? start<T, 64>(a, maps, max_q, stream) : start<T, 32>(a, maps, max_q, stream);
 }
 
 }  // namespace
@@ -481,7 +489,7 @@ cudaError_t launch_attn_tc(const AttnArgs &a, int type, uint32_t max_q, bool *ta
         !map_rows(&maps.v, a.v, type, a.kv_rows, a.v_row, a.kv_heads, a.v_head, a.d))
         return cudaSuccess;  // strides the encoder does not take
     *taken = true;
-    return type == PPOCR_F16 ? start<__half>(a, maps, max_q, stream) : start<__nv_bfloat16>(a, maps, max_q, stream);
+    return type == PPOCR_F16 ? start_d<__half>(a, maps, max_q, stream) : start_d<__nv_bfloat16>(a, maps, max_q, stream);
 }
 
 }  // namespace ppocr
