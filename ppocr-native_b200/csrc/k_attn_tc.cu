@@ -54,23 +54,56 @@ __device__ __forceinline__ uint32_t idesc(int n, int b_major) {
     return (1u << 4) | (F << 7) | (F << 10) | (uint32_t(b_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(BQ >> 4) << 24);
 }
 
-// Issued where `on` is true: a predicate and no branch, so that the operands
-// stay in uniform registers.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t on) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(on));
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc, uint32_t on) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(on));
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
 }
-__device__ __forceinline__ void commit(uint32_t bar, uint32_t on) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on)
-        : "memory");
+
+// The products of one tile, their number known at compile time and nothing
+// between them: 32 + N / 4 cycles each with both operands in shared memory (its
+// bandwidth), N / 2 with one in tensor memory; a branch or a predicate a
+// product cost 11 to 43 more.
+template <int STEPS, int BK>
+__device__ __forceinline__ void score_steps(uint32_t d, uint64_t q, uint64_t k, uint32_t id) {
+#pragma unroll
+    for (int kk = 0; kk < STEPS; kk++)  // the descriptors' addresses count 16 bytes: 16 columns are 2, a panel all its rows
+        mma_ss(d, q + (kk >> 2) * (BQ * 128 / 16) + (kk & 3) * 2, k + (kk >> 2) * (BK * 128 / 16) + (kk & 3) * 2, id, kk > 0);
+}
+template <int BK>
+__device__ __forceinline__ void score_product(int steps, uint32_t d, uint64_t q, uint64_t k, uint32_t id) {
+    switch (steps) {
+    case 1: return score_steps<1, BK>(d, q, k, id);
+    case 2: return score_steps<2, BK>(d, q, k, id);
+    case 3: return score_steps<3, BK>(d, q, k, id);
+    case 4: return score_steps<4, BK>(d, q, k, id);
+    case 5: return score_steps<5, BK>(d, q, k, id);
+    case 6: return score_steps<6, BK>(d, q, k, id);
+    case 7: return score_steps<7, BK>(d, q, k, id);
+    default: return score_steps<8, BK>(d, q, k, id);
+    }
+}
+template <int STEPS>
+__device__ __forceinline__ void value_steps(uint32_t d, uint32_t p, uint64_t v, uint32_t id, uint32_t acc) {
+#pragma unroll
+    for (int kk = 0; kk < STEPS; kk++) mma_ts(d, p + kk * 8, v + kk * 128, id, kk > 0 ? 1 : acc);
+}
+__device__ __forceinline__ void value_product(int steps, uint32_t d, uint32_t p, uint64_t v, uint32_t id, uint32_t acc) {
+    switch (steps) {
+    case 1: return value_steps<1>(d, p, v, id, acc);
+    case 2: return value_steps<2>(d, p, v, id, acc);
+    case 3: return value_steps<3>(d, p, v, id, acc);
+    default: return value_steps<4>(d, p, v, id, acc);
+    }
+}
+
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float *v) {
@@ -274,14 +307,11 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                 const auto scores = [&](int it) {
                     on &= __all_sync(0xffffffffu, wait(k_bar + buf(it) * 8, phase(it)));
                     fence_after();
-                    const uint32_t id_s = idesc<T>((tl.count(it) + 15) / 16 * 16, 0), go = one && on;
-                    const uint64_t k_at = k_desc + buf(it) * next;
-#pragma unroll
-                    for (int kk = 0; kk < 8; kk++) {
-                        const uint64_t q_in = (kk >> 2) * (BQ * 128 / 16) + (kk & 3) * 2, k_in = (kk >> 2) * (BK * 128 / 16) + (kk & 3) * 2;
-                        mma_ss(tmem + buf(it) * BK, q_desc + q_in, k_at + k_in, id_s, kk > 0, go & uint32_t(kk < steps));
+                    const uint32_t id_s = idesc<T>((tl.count(it) + 15) / 16 * 16, 0);
+                    if (one && on) {
+                        score_product<BK>(steps, tmem + buf(it) * BK, q_desc, k_desc + buf(it) * next, id_s);
+                        commit(s_bar + buf(it) * 8);
                     }
-                    commit(s_bar + buf(it) * 8, go);
                 };
                 scores(0);
                 for (int it = 0; it < tl.n; it++) {
@@ -289,13 +319,10 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                     const int n = (tl.count(it) + 15) / 16;
                     on &= __all_sync(0xffffffffu, wait(v_bar + buf(it) * 8, phase(it)) && wait(p_bar + buf(it) * 8, phase(it)));
                     fence_after();
-                    const uint32_t go = one && on;
-                    const uint64_t v_at = v_desc + buf(it) * next;
-#pragma unroll
-                    for (int kk = 0; kk < BK / 16; kk++)
-                        mma_ts(tmem + O_COL, tmem + buf(it) * BK + kk * 8, v_at + uint64_t(kk * 128), id_o, it > 0 || kk > 0,
-                               go & uint32_t(kk < n));
-                    commit(o_bar + buf(it) * 8, go);
+                    if (one && on) {
+                        value_product(n, tmem + O_COL, tmem + buf(it) * BK, v_desc + buf(it) * next, id_o, it > 0);
+                        commit(o_bar + buf(it) * 8);
+                    }
                 }
             }
             __syncwarp();
