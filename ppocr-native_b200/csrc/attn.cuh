@@ -26,6 +26,7 @@ struct AttnArgs {
     int left, right, sinks;  // left, right -1: no limit
     float scale_log2;  // the scale times log2 e
     int q_bytes, k_bytes, v_bytes;  // widest copy each tensor's rows allow: 16, 4 or 2 bytes
+    int sort;                        // split form: take the lanes by their keys, most first
     int out_vec;                     // 1 when pairs of outputs may be stored together, 2 when 16 bytes may
 };
 
@@ -83,35 +84,53 @@ struct KeyTiles {
 };
 
 // Rows [0, rows) of a tensor's one head into a shared tile of ROWS rows of
-// STRIDE elements, zeros past `rows` and past d, by `threads` threads.
-template <class T, int ROWS, int DP, int STRIDE, int W>
-__device__ __forceinline__ void load_rows_w(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int tid,
-                                            int threads) {
+// STRIDE elements, zeros past `rows` and past d, by THREADS threads.
+template <class T, int ROWS, int DP, int STRIDE, int W, int THREADS>
+__device__ __forceinline__ void load_rows_w(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int tid) {
     constexpr int E = W / int(sizeof(T)), CPR = DP / E;
-    for (int e = tid; e < ROWS * CPR; e += threads) {
-        const int r = e / CPR, c = e % CPR;
-        const int left = r < rows ? (d - c * E) * int(sizeof(T)) : 0;
-        const int valid = left < 0 ? 0 : left > W ? W : left;
-        const T *from = valid ? src + r * row_stride + c * E : src;
-        const uint32_t to = dst + uint32_t((r * STRIDE + c * E) * int(sizeof(T)));
-        if constexpr (W >= 4) {
-            copy_async<W>(to, from, valid);
+    if constexpr (W >= 4 && THREADS % CPR == 0 && ROWS % (THREADS / CPR) == 0) {
+        // a thread's copies lie in one column, THREADS / CPR rows apart
+        constexpr int STEP = THREADS / CPR;
+        const int r0 = tid / CPR, c = tid % CPR * E;
+        const int left = (d - c) * int(sizeof(T)), valid = left < 0 ? 0 : left > W ? W : left;
+        const T *from = src + r0 * row_stride + c;
+        uint32_t to = dst + uint32_t((r0 * STRIDE + c) * int(sizeof(T)));
+        const int64_t step = STEP * row_stride;
+        if (rows == ROWS && d == DP) {
+#pragma unroll
+            for (int i = 0; i < ROWS / STEP; i++, from += step) copy_async<W>(to + uint32_t(i * STEP * STRIDE * int(sizeof(T))), from, W);
         } else {
-            uint16_t v = 0;
-            if (valid) v = __ldg(reinterpret_cast<const uint16_t *>(from));
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+#pragma unroll
+            for (int i = 0; i < ROWS / STEP; i++, from += step) {
+                const int v = r0 + i * STEP < rows ? valid : 0;
+                copy_async<W>(to + uint32_t(i * STEP * STRIDE * int(sizeof(T))), v ? from : src, v);
+            }
+        }
+    } else {
+        for (int e = tid; e < ROWS * CPR; e += THREADS) {
+            const int r = e / CPR, c = e % CPR;
+            const int left = r < rows ? (d - c * E) * int(sizeof(T)) : 0;
+            const int valid = left < 0 ? 0 : left > W ? W : left;
+            const T *from = valid ? src + r * row_stride + c * E : src;
+            const uint32_t to = dst + uint32_t((r * STRIDE + c * E) * int(sizeof(T)));
+            if constexpr (W >= 4) {
+                copy_async<W>(to, from, valid);
+            } else {
+                uint16_t v = 0;
+                if (valid) v = __ldg(reinterpret_cast<const uint16_t *>(from));
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+            }
         }
     }
 }
-template <class T, int ROWS, int DP, int STRIDE>
-__device__ __forceinline__ void load_rows(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int bytes,
-                                          int tid, int threads) {
+template <class T, int ROWS, int DP, int STRIDE, int THREADS>
+__device__ __forceinline__ void load_rows(uint32_t dst, const T *src, int64_t row_stride, int rows, int d, int bytes, int tid) {
     if (bytes == 16)
-        load_rows_w<T, ROWS, DP, STRIDE, 16>(dst, src, row_stride, rows, d, tid, threads);
+        load_rows_w<T, ROWS, DP, STRIDE, 16, THREADS>(dst, src, row_stride, rows, d, tid);
     else if (sizeof(T) == 4 || bytes == 4)
-        load_rows_w<T, ROWS, DP, STRIDE, 4>(dst, src, row_stride, rows, d, tid, threads);
+        load_rows_w<T, ROWS, DP, STRIDE, 4, THREADS>(dst, src, row_stride, rows, d, tid);
     else if constexpr (sizeof(T) == 2)
-        load_rows_w<T, ROWS, DP, STRIDE, 2>(dst, src, row_stride, rows, d, tid, threads);
+        load_rows_w<T, ROWS, DP, STRIDE, 2, THREADS>(dst, src, row_stride, rows, d, tid);
 }
 
 // Row strides of the shared tiles, padded so that a fragment's 32 accesses

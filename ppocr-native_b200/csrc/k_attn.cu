@@ -47,15 +47,12 @@ __global__ void __launch_bounds__(ROW_THREADS, RowTile<T, DP>::BLOCKS) attn_rows
         kt.plan<BK>(a, p0, p1, ln.nk);
         const auto fetch = [&](int it, int buf) {
             const int j = kt.first<BK>(it), n = min(BK, kt.end(it) - j);
-            load_rows<T, BK, DP, STRIDE>(kv + buf * 2 * R::K_BYTES, k + j * a.k_row, a.k_row, n, a.d, a.k_bytes, tid,
-                                         ROW_THREADS);
-            load_rows<T, BK, DP, STRIDE>(kv + (buf * 2 + 1) * R::K_BYTES, v + j * a.v_row, a.v_row, n, a.d, a.v_bytes,
-                                         tid, ROW_THREADS);
+            load_rows<T, BK, DP, STRIDE, ROW_THREADS>(kv + buf * 2 * R::K_BYTES, k + j * a.k_row, a.k_row, n, a.d, a.k_bytes, tid);
+            load_rows<T, BK, DP, STRIDE, ROW_THREADS>(kv + (buf * 2 + 1) * R::K_BYTES, v + j * a.v_row, a.v_row, n, a.d, a.v_bytes, tid);
         };
         __syncthreads();  // the last tile's readers are done
-        load_rows<T, BQ, DP, STRIDE>(
-            qs, static_cast<const T *>(a.q) + (ln.q0 + i0) * a.q_row + h * a.q_head, a.q_row, rows, a.d, a.q_bytes, tid,
-            ROW_THREADS);
+        load_rows<T, BQ, DP, STRIDE, ROW_THREADS>(qs, static_cast<const T *>(a.q) + (ln.q0 + i0) * a.q_row + h * a.q_head, a.q_row,
+                                                  rows, a.d, a.q_bytes, tid);
         if (kt.n > 0) fetch(0, 0);
         copy_commit();
 
