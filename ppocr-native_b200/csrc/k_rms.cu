@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "block.cuh"
+#include "devmath.cuh"
 
 namespace ppocr {
 
@@ -26,8 +27,8 @@ struct RmsArgs {
     uint8_t *y;
     float *scales;
     int64_t rows, x_row, r_row, sum_row, y_row;
-    int channels, group, groups;
-    float eps;
+    int channels, group, group_log2, groups;
+    float eps, inv_channels;
 };
 
 // A lane's 8 channels of one chunk as they lie in memory.
@@ -102,17 +103,17 @@ struct Eight {
     }
 };
 
-// |v| as bits: as integers they order as the magnitudes do, infinity above
-// every number and NaN above infinity, so a NaN is never lost.
-__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-// What a group of this peak magnitude is multiplied by for its 8 bits, one
-// over its scale. The scale is rounded to f32 (and may fall to zero), so the
-// quotient by it is taken where 448 / peak would overflow; zero for zeros.
-__device__ __forceinline__ float steps_of(uint32_t peak) {
-    const float p = __uint_as_float(peak);
-    if (p < 1e-30f) return p / 448.0f == 0.0f ? 0.0f : fminf(1.0f / (p / 448.0f), 3e38f);
-    return 448.0f / p;
+// The larger magnitude of three; a NaN is never lost, and as an integer lies
+// above every other magnitude's bits.
+__device__ __forceinline__ float peak3(float top, float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(top), "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+__device__ __forceinline__ float peak2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
 // Two values as e4m3, the first in the low byte.
@@ -120,10 +121,26 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// What the chunk's v = s * gamma are multiplied by for their 8 bits, from their
+// group's peak magnitude of n = v * inv: inv * 448 / peak. Where that quotient
+// leaves the quick division's range (or there is none: zeros, NaN), v becomes
+// n first; a scale that f32 rounds to zero gives zeros.
+__device__ __forceinline__ float steps_of(float peak, float inv, float v[8]) {
+    if (peak > 1e-30f && peak < 1e37f) return __fdividef(448.0f, peak) * inv;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= inv;
+    if (peak <= 1e-30f) return peak * (1.0f / 448.0f) == 0.0f ? 0.0f : fminf(1.0f / (peak * (1.0f / 448.0f)), 3e38f);
+    return 448.0f / peak;
+}
+
 // TPR threads a row, CH chunks of 8 channels a thread. Rows narrower than a
 // warp's reach share a block of 128 threads, four rows to it. A block walks
 // rows gridDim apart and has the next row's loads in flight while it works
 // on this one.
+//
+// The 8 bits are those of v = s * gamma over its own peak: the root-mean-square
+// reaches the scale alone, so a row needs one barrier, for the sum of squares
+// and (one scale a row) the peak together.
 //
 // VEC: a chunk is 8 consecutive channels, 16-byte loads; else (rows, strides
 // or bases that 16 bytes do not divide) channels 32 apart, so that a warp's
@@ -131,167 +148,166 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
 template <class T, int TPR, int CH, bool VEC>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const __grid_constant__ RmsArgs a) {
     constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, WARPS = TPR / 32;
-    __shared__ float part[WARPS];
-    __shared__ uint32_t peak[WARPS];
+    // two rows' in turn: between two writes of one lies the other's barrier
+    __shared__ float part[2][WARPS], peak[2][WARPS];
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = t / 32;
     const auto place = [&](int c) { return VEC ? (c * TPR + t) * 8 : (c * TPR + (t & ~31)) * 8 + lane; };
     const T *x = static_cast<const T *>(a.x), *r = static_cast<const T *>(a.r);
     Eight<T> nx[CH], nr[CH];
     const auto fetch = [&](int64_t row) {
         if (row >= a.rows) return;
+        const T *xr = x + row * a.x_row, *rr = r + row * a.r_row;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int at = place(c);
             if constexpr (VEC) {
                 if (at < a.channels) {
-                    nx[c].load(x + row * a.x_row + at);
-                    if (r) nr[c].load(r + row * a.r_row + at);
+                    nx[c].load(xr + at);
+                    if (r) nr[c].load(rr + at);
                 }
             } else {
-                nx[c].load_apart(x + row * a.x_row + at, a.channels - at);
-                if (r) nr[c].load_apart(r + row * a.r_row + at, a.channels - at);
+                nx[c].load_apart(xr + at, a.channels - at);
+                if (r) nr[c].load_apart(rr + at, a.channels - at);
             }
         }
     };
     int64_t row = int64_t(blockIdx.x) * ROWS + threadIdx.x / TPR;
     fetch(row);
+    int turn = 0;
     for (int64_t row0 = int64_t(blockIdx.x) * ROWS; row0 < a.rows; row0 += int64_t(gridDim.x) * ROWS) {
         const int channels = row < a.rows ? a.channels : 0;  // of this row: none past the last
-        float s[CH][8], square = 0.0f;
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-            if (place(c) < channels) {
-                nx[c].get(s[c]);
-                if (r) {
-                    float v[8];
-                    nr[c].get(v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s[c][i] += v[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) s[c][i] = 0.0f;
-            }
-        }
-        fetch(row + int64_t(gridDim.x) * ROWS);
-#pragma unroll
-        for (int c = 0; c < CH; c++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) square = fmaf(s[c][i], s[c][i], square);
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
-        if constexpr (WARPS > 1) {
-            if (lane == 0) part[warp] = square;
-            __syncthreads();
-            square = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WARPS; w++) square += part[w];
-        }
-        if (a.sum) {
-            T *sum = static_cast<T *>(a.sum) + row * a.sum_row;
-#pragma unroll
-            for (int c = 0; c < CH; c++) {
-                if (place(c) >= channels) continue;
-                Eight<T> e;
-                e.put(s[c]);
-                if constexpr (VEC)
-                    e.store(sum + place(c));
-                else
-                    e.store_apart(sum + place(c), channels - place(c));
-            }
-        }
-        const float inv = 1.0f / sqrtf(square / float(a.channels) + a.eps);
-        uint32_t top[CH][VEC ? 1 : 8], all = 0;
+        float v[CH][8], top[CH][VEC ? 1 : 8];
+        float2 square2 = make_float2(0.0f, 0.0f);
+        T *sum = static_cast<T *>(a.sum) + row * a.sum_row;
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int at = place(c);
-            if constexpr (VEC) {
-                top[c][0] = 0;
-                if (at < channels) {
+            if constexpr (VEC) top[c][0] = 0.0f;
+            if (at < channels) {
+                nx[c].get(v[c]);
+                if (r) {
+                    float w[8];
+                    nr[c].get(w);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[c][i] += w[i];
+                }
+                if (a.sum) {
+                    Eight<T> e;
+                    e.put(v[c]);
+                    if constexpr (VEC)
+                        e.store(sum + at);
+                    else
+                        e.store_apart(sum + at, channels - at);
+                }
+                float gamma[8];
+                if constexpr (VEC) {
                     const float4 g0 = __ldg(reinterpret_cast<const float4 *>(a.gamma + at));
                     const float4 g1 = __ldg(reinterpret_cast<const float4 *>(a.gamma + at) + 1);
-                    const float gamma[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+                    gamma[0] = g0.x, gamma[1] = g0.y, gamma[2] = g0.z, gamma[3] = g0.w;
+                    gamma[4] = g1.x, gamma[5] = g1.y, gamma[6] = g1.z, gamma[7] = g1.w;
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        s[c][i] = s[c][i] * inv * gamma[i];
-                        top[c][0] = max(top[c][0], mag(s[c][i]));
-                    }
+                    for (int i = 0; i < 8; i++) gamma[i] = at + i * 32 < channels ? __ldg(a.gamma + at + i * 32) : 0.0f;
                 }
-                all = max(all, top[c][0]);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float2 s = make_float2(v[c][i], v[c][i + 1]);
+                    square2 = ffma2(s, s, square2);
+                    v[c][i] *= gamma[i];
+                    v[c][i + 1] *= gamma[i + 1];
+                    if constexpr (VEC)
+                        top[c][0] = peak3(top[c][0], v[c][i], v[c][i + 1]);
+                    else
+                        top[c][i] = fabsf(v[c][i]), top[c][i + 1] = fabsf(v[c][i + 1]);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    s[c][i] = at + i * 32 < channels ? s[c][i] * inv * __ldg(a.gamma + at + i * 32) : 0.0f;
-                    top[c][i] = mag(s[c][i]);
-                    all = max(all, top[c][i]);
+                    v[c][i] = 0.0f;
+                    if constexpr (!VEC) top[c][i] = 0.0f;
                 }
             }
         }
-        float *scales = a.scales + row * a.groups;
-        if (a.group == 0) {
-            all = __reduce_max_sync(0xffffffffu, all);
-            if constexpr (WARPS > 1) {
-                if (lane == 0) peak[warp] = all;
-                __syncthreads();
-                all = 0;
+        fetch(row + int64_t(gridDim.x) * ROWS);
+        float square = square2.x + square2.y;
 #pragma unroll
-                for (int w = 0; w < WARPS; w++) all = max(all, peak[w]);
+        for (int d = 16; d; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+        float all = 0.0f;
+        if (a.group == 0) {
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                if constexpr (VEC)
+                    all = peak2(all, top[c][0]);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) all = peak3(all, top[c][i], top[c][i + 1]);
             }
-            if (channels && t == 0) scales[0] = __uint_as_float(all) / 448.0f;
+            all = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(all)));
         } else {
 #pragma unroll
             for (int c = 0; c < CH; c++) {
                 if constexpr (VEC) {
                     // a group of 32, 64 or 128 channels is 4, 8 or 16 neighbouring lanes' chunks
-                    uint32_t &m = top[c][0];
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    if (a.group > 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    if (a.group > 64) m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    if (place(c) < channels && (place(c) & (a.group - 1)) == 0)
-                        scales[place(c) / a.group] = __uint_as_float(m) / 448.0f;
+                    float &m = top[c][0];
+                    m = peak2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = peak2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    if (a.group > 32) m = peak2(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    if (a.group > 64) m = peak2(m, __shfl_xor_sync(0xffffffffu, m, 8));
                 } else {
                     // 1, 2 or 4 of the warp's 32-channel runs
 #pragma unroll
-                    for (int i = 0; i < 8; i++) top[c][i] = __reduce_max_sync(0xffffffffu, top[c][i]);
+                    for (int i = 0; i < 8; i++) top[c][i] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top[c][i])));
 #pragma unroll
                     for (int i = 0; i < 8; i += 2)
-                        if (a.group > 32) top[c][i] = top[c][i + 1] = max(top[c][i], top[c][i + 1]);
+                        if (a.group > 32) top[c][i] = top[c][i + 1] = peak2(top[c][i], top[c][i + 1]);
 #pragma unroll
                     for (int i = 0; i < 8; i += 4)
-                        if (a.group > 64) top[c][i] = top[c][i + 1] = top[c][i + 2] = top[c][i + 3] = max(top[c][i], top[c][i + 2]);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int at = place(c) + i * 32;
-                        if (lane == 0 && at < channels && (at & (a.group - 1)) == 0)
-                            scales[at / a.group] = __uint_as_float(top[c][i]) / 448.0f;
-                    }
+                        if (a.group > 64) top[c][i] = top[c][i + 1] = top[c][i + 2] = top[c][i + 3] = peak2(top[c][i], top[c][i + 2]);
                 }
             }
         }
+        if constexpr (WARPS > 1) {
+            if (lane == 0) part[turn][warp] = square, peak[turn][warp] = all;
+            __syncthreads();
+            square = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) square += part[turn][w];
+            if (a.group == 0) {
+#pragma unroll
+                for (int w = 0; w < WARPS; w++) all = peak2(all, peak[turn][w]);
+            }
+            turn ^= 1;
+        }
+        const float inv = rsqrtf(fmaf(square, a.inv_channels, a.eps));
+        float *scales = a.scales + row * a.groups;
         uint8_t *y = a.y + row * a.y_row;
+        if (a.group == 0 && channels && t == 0) scales[0] = all * inv * (1.0f / 448.0f);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
-            const int n = channels - place(c);
+            const int at = place(c), n = channels - at;
+            if (n <= 0) continue;
             if constexpr (VEC) {
-                if (n <= 0) continue;
-                const float f = steps_of(a.group ? top[c][0] : all);
+                const float p = (a.group ? top[c][0] : all) * inv;
+                if (a.group && (at & (a.group - 1)) == 0) scales[at >> a.group_log2] = p * (1.0f / 448.0f);
+                const float f = steps_of(p, inv, v[c]);
                 uint32_t w[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++)
-                    w[i] = e4m3_pair(s[c][4 * i] * f, s[c][4 * i + 1] * f) |
-                           e4m3_pair(s[c][4 * i + 2] * f, s[c][4 * i + 3] * f) << 16;
-                *reinterpret_cast<uint2 *>(y + place(c)) = make_uint2(w[0], w[1]);
+                    w[i] = e4m3_pair(v[c][4 * i] * f, v[c][4 * i + 1] * f) |
+                           e4m3_pair(v[c][4 * i + 2] * f, v[c][4 * i + 3] * f) << 16;
+                *reinterpret_cast<uint2 *>(y + at) = make_uint2(w[0], w[1]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i * 32 < n) y[place(c) + i * 32] = uint8_t(e4m3_pair(s[c][i] * steps_of(a.group ? top[c][i] : all), 0.0f));
+                for (int i = 0; i < 8; i++) {
+                    if (i * 32 >= n) continue;
+                    const float p = (a.group ? top[c][i] : all) * inv;
+                    if (a.group && lane == 0 && ((at + i * 32) & (a.group - 1)) == 0) scales[(at + i * 32) >> a.group_log2] = p * (1.0f / 448.0f);
+                    float one[8] = {v[c][i]};
+                    const float f = steps_of(p, inv, one);
+                    y[at + i * 32] = uint8_t(e4m3_pair(one[0] * f, 0.0f));
+                }
             }
         }
-        // the next row's sums go where every warp has read this one's by now:
-        // between two uses of `part`, and of `peak`, lies a barrier of the other
-        if (WARPS > 1 && a.group != 0) __syncthreads();
         row += int64_t(gridDim.x) * ROWS;
     }
 }
@@ -355,7 +371,8 @@ extern "C" int ppocr_rms_norm_e4m3(const ppocr_rms_norm_shape *s, const void *x,
     if (s->rows > 1 && (a.sum_row < int64_t(c) || a.y_row < int64_t(c)))
         return refuse(PPOCR_E_ARG, me, "output rows overlap");
     a.channels = int(c), a.group = int(s->group), a.groups = s->group ? int((c + s->group - 1) / s->group) : 1;
-    a.eps = s->eps;
+    a.group_log2 = s->group == 128 ? 7 : s->group == 64 ? 6 : 5;
+    a.eps = s->eps, a.inv_channels = 1.0f / float(c);
     // outputs may meet the inputs only as x or residual updated in place
     const auto span = [&](int64_t row) { return (s->rows - 1) * uint64_t(row) + c; };
     const uint64_t xn = span(a.x_row) * size, rn = residual ? span(a.r_row) * size : 0, sn = sum ? span(a.sum_row) * size : 0;
