@@ -115,21 +115,20 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
     in.begin(a, at);
     uint4 xf[SL][4][CT];
     const auto load = [&](int c0) {
+        const auto k_of = [&](int c, int u) { return (c0 + c) * 128 + (BPG == 4 ? at.t * 32 + u * 8 : u * 32 + at.t * 8); };
 #pragma unroll
         for (int c = 0; c < SL; c++)
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int k = (c0 + c) * 128 + (BPG == 4 ? at.t * 32 + u * 8 : u * 32 + at.t * 8);
+            for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
                     const int col = ct * 8 + at.g, r = col / PARTS;
-                    xf[c][u][ct] = make_uint4(0, 0, 0, 0);
-                    if (r >= rows || c0 + c >= at.c_hi) continue;
+                    const bool there = r < rows && c0 + c < at.c_hi;
                     if constexpr (PARTS == 1) {
-                        xf[c][u][ct] = load_pairs<XT>(a, m0 + r, k);
+                        xf[c][u][ct] = take_x<XT>(a, m0 + r, k_of(c, u), there);
                     } else {
-                        float v[8];
-                        load_x<XT>(a, m0 + r, k, v);
+                        float v[8] = {};
+                        if (there) load_x<XT>(a, m0 + r, k_of(c, u), v);
                         uint32_t p[4];
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -137,7 +136,14 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                         xf[c][u][ct] = make_uint4(p[0], p[1], p[2], p[3]);
                     }
                 }
-            }
+        if constexpr (PARTS == 1) {
+#pragma unroll
+            for (int c = 0; c < SL; c++)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) xf[c][u][ct] = pairs_of<XT>(xf[c][u][ct]);
+        }
     };
     const auto value = [&](int l, int tile, int m, int r) {
         const float *from = red + (((l * a.depth + tile % a.depth) * warps + tile / a.depth * a.wk) * 16 + r) * WIDE + m * PARTS;
@@ -146,10 +152,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
             for (int w = 0; w < a.wk; w++) y += from[w * 16 * WIDE + p];
         return y;
     };
-    const auto finish = [&](int m, int n, float y) {
-        if (sizeof(XT) == 1 && a.x_groups == 1) y *= __ldg(a.x_scales + m0 + m);
-        put_y(a, m0 + m, n, y);
-    };
+    const auto finish = [&](int m, int n, float y, float bias, float scale) { put_y(a, m0 + m, n, fmaf(y, scale, bias)); };
     for (int b0 = 0; b0 < at.lists; b0 += a.batch) {
         const int count = min(a.batch, at.lists - b0);
         for (int lap = 0; lap < a.laps; lap++) {
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                     for (int j = 0; j < SL * 4 / BPG; j++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            s[j / (4 / BPG)][j % (4 / BPG)][h] = in.scale(d, j, at.g + 8 * h) * Enter<XT>::SCALE;
+                            s[j / (4 / BPG)][j % (4 / BPG)][h] = in.scale(a, d, j, at.g + 8 * h) * Enter<XT>::SCALE;
                             z[j / (4 / BPG)][j % (4 / BPG)][h] = in.zero(d, j, at.g + 8 * h);
                         }
                     in.scales(a, at, d);
@@ -215,6 +218,22 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                         }
                         in.chunk(a, at, d, c);
                     }
+                    const float bias[2] = {in.b[d][0], in.b[d][1]};
+                    in.biases(a, at, d);
+                    if (PARTS == 1 && a.direct) {
+                        // this warp's sums are whole: out with them
+                        const int n0 = at.row(a, b0 + i, at.r_warp) + d * 16 + at.g;
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int n = n0 + 8 * (e >> 1), m = ct * 8 + at.t * 2 + (e & 1);
+                                if (n >= a.n || m >= rows) continue;
+                                const float scale = sizeof(XT) == 1 && a.x_groups == 1 ? __ldg(a.x_scales + m0 + m) : 1.0f;
+                                finish(m, n, acc[ct][e], bias[e >> 1], scale);
+                            }
+                        continue;
+                    }
                     float *mine = red + (((i * a.depth + d) * warps + at.warp) * 16 + at.g) * WIDE + at.t * 2;
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++)
@@ -229,7 +248,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                 in.next(a, at);
             }
         }
-        join(a, at, rows, b0, count, red + a.red_floats, value, finish);
+        if (!a.direct) join(a, at, m0, rows, b0, count, red + a.red_floats, value, finish);
     }
 }
 
@@ -240,7 +259,7 @@ cudaError_t start(Q4Args a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     a.cols_rows = Q::COLS / Enter<XT>::PARTS < a.m ? Q::COLS / Enter<XT>::PARTS : a.m;
     return launch_q4(reinterpret_cast<const void *>(q4_kernel<XT, CT, BPG, ZEROS>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, Q::WIDE, 0,
-                     Q::SHARED, stream);
+                     Q::SHARED, Enter<XT>::PARTS == 1, stream);
 }
 
 template <class XT, int BPG, bool ZEROS>

@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
         for (int w = 0; w < a.wk; w++) y += from[w * ROWS_X * 16];
         return y;
     };
-    const auto finish = [&](int m, int n, float y) {
+    const auto finish = [&](int m, int n, float y, float bias, float) {
         if (!(fabsf(y) < INFINITY)) y = plain_q4<XT>(a, m, n);
-        put_y(a, m, n, y);
+        put_y(a, m, n, y + bias);
     };
     for (int b0 = 0; b0 < at.lists; b0 += a.batch) {
         const int count = min(a.batch, at.lists - b0);
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                     for (int j = 0; j < SL * GPC; j++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            s[j][h] = in.scale(d, j, at.g + 8 * h);
+                            s[j][h] = in.scale(a, d, j, at.g + 8 * h);
                             z[j][h] = in.zero(d, j, at.g + 8 * h);
                         }
                     in.scales(a, at, d);
@@ -199,6 +199,8 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                         }
                         in.chunk(a, at, d, c);
                     }
+                    const float bias[2] = {in.b[d][0], in.b[d][1]};
+                    in.biases(a, at, d);
                     // columns 2t and 2t + 1 are bytes 0, 1 (t even) or 2, 3 of a row: one number
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -207,7 +209,10 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                         y += __shfl_xor_sync(0xffffffffu, y, 1);
                         y = y * back0 * back1;
                         const int m = at.t >> 1;
-                        if ((at.t & 1) == 0 && m < ROWS_X) {
+                        if ((at.t & 1) == 0 && m < ROWS_X && a.direct) {
+                            const int n = at.row(a, b0 + i, at.r_warp) + d * 16 + at.g + 8 * h;
+                            if (n < a.n) finish(m, n, y, bias[h], 1.0f);
+                        } else if ((at.t & 1) == 0 && m < ROWS_X) {
                             float *to = red + (((i * a.depth + d) * warps + at.warp) * ROWS_X + m) * 16 + at.g + 8 * h;
                             *to = lap > 0 ? *to + y : y;
                         }
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                 in.next(a, at);
             }
         }
-        join(a, at, ROWS_X, b0, count, red + a.red_floats, value, finish);
+        if (!a.direct) join(a, at, 0, ROWS_X, b0, count, red + a.red_floats, value, finish);
     }
 }
 
@@ -227,7 +232,7 @@ cudaError_t start(Q4Args a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     a.cols_rows = a.m;
     return launch_q4(reinterpret_cast<const void *>(q4_int_kernel<XT, BPG, ZEROS, ROWS_X>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, ROWS_X,
-                     Q::SL * 4 * 4 * ROWS_X * 32, Q::SHARED, stream);
+                     Q::SL * 4 * 4 * ROWS_X * 32, Q::SHARED, true, stream);
 }
 
 template <class XT, int BPG>

@@ -43,6 +43,7 @@ struct Q4Args {
     int cols_rows;            // rows of x a pass takes
     int ks, wk;               // blocks of a cluster, and warps of a block, that share a tile
     int chunks, share, laps;  // chunks of 128 k in all and in a block's share; slices a warp takes of it
+    bool direct;              // a warp has the whole sum of its tiles: no join
     int depth;                // tiles of an item
     int batch;                // lists of tiles between two joins
     int red_floats, stage_floats;  // of partial sums in shared memory before the cluster's, and before what else a warp keeps there
@@ -57,6 +58,16 @@ struct e4m3 {
     uint8_t bits;
 };
 
+// A scale's bits, and the number they are: the bits are taken ahead, the number
+// where it is used, so that no load is waited for before it is needed.
+__device__ __forceinline__ uint32_t scale_bits(const Q4Args &a, int64_t at) {
+    if (a.scale_type == PPOCR_F32) return __ldg(static_cast<const uint32_t *>(a.scales) + at);
+    return __ldg(static_cast<const unsigned short *>(a.scales) + at);
+}
+__device__ __forceinline__ float scale_of(const Q4Args &a, uint32_t bits) {
+    if (a.scale_type == PPOCR_F16) return __half2float(__ushort_as_half((unsigned short)bits));
+    return __uint_as_float(a.scale_type == PPOCR_BF16 ? bits << 16 : bits);
+}
 __device__ __forceinline__ float load_scale(const Q4Args &a, int64_t at) {
     if (a.scale_type == PPOCR_F16) return __half2float(static_cast<const __half *>(a.scales)[at]);
     if (a.scale_type == PPOCR_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.scales)[at]);
@@ -101,31 +112,43 @@ __device__ __forceinline__ void load_x(const Q4Args &a, int row, int k, float v[
     }
 }
 
-// The same eight as pairs (0, 4), (1, 5), (2, 6), (3, 7) of the matrix
-// instruction's type, for types that enter in one part.
+// Eight values of x as they lie in memory, of a type that enters in one part
+// (zeros past k), and as pairs (0, 4), (1, 5), (2, 6), (3, 7) of the matrix
+// instruction's type: two steps, so that a warp's loads all go out first.
 template <class XT>
-__device__ __forceinline__ uint4 load_pairs(const Q4Args &a, int row, int k) {
-    uint32_t u[4];  // pairs (0, 1), (2, 3), (4, 5), (6, 7)
+__device__ __forceinline__ uint4 take_x(const Q4Args &a, int row, int k, bool there) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (!there || k >= a.k) return v;
+    const XT *p = static_cast<const XT *>(a.x) + row * a.x_row + k;
     if (a.x_vec && k + 8 <= a.k) {
-        const XT *p = static_cast<const XT *>(a.x) + row * a.x_row + k;
         if constexpr (sizeof(XT) == 2) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-            u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+            v = __ldg(reinterpret_cast<const uint4 *>(p));
         } else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const __half2_raw h =
-                    __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t((i < 2 ? v.x : v.y) >> (16 * (i & 1))), __NV_E4M3);
-                u[i] = *reinterpret_cast<const uint32_t *>(&h);
-            }
+            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+            v.x = u.x, v.y = u.y;
         }
-    } else {
-        float v[8];
-        load_x<XT>(a, row, k, v);
-        using M = typename std::conditional<sizeof(XT) == 1, __half, XT>::type;
+        return v;
+    }
+    uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = pack2<M>(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < 8; i++)
+        if (k + i < a.k) {
+            if constexpr (sizeof(XT) == 2)
+                u[i / 2] |= uint32_t(reinterpret_cast<const unsigned short *>(p)[i]) << (16 * (i & 1));
+            else
+                u[i / 4] |= uint32_t(reinterpret_cast<const unsigned char *>(p)[i]) << (8 * (i & 3));
+        }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <class XT>
+__device__ __forceinline__ uint4 pairs_of(const uint4 &v) {
+    uint32_t u[4] = {v.x, v.y, v.z, v.w};  // pairs (0, 1), (2, 3), (4, 5), (6, 7)
+    if constexpr (sizeof(XT) == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t((i < 2 ? v.x : v.y) >> (16 * (i & 1))), __NV_E4M3);
+            u[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
     }
     return make_uint4(__byte_perm(u[0], u[2], 0x5410), __byte_perm(u[0], u[2], 0x7632), __byte_perm(u[1], u[3], 0x5410),
                       __byte_perm(u[1], u[3], 0x7632));
@@ -190,19 +213,20 @@ struct Stream {
     static constexpr int NG = SL * 4 / BPG;         // groups a slice
     static constexpr int NS = NG < 2 ? 1 : NG / 2;  // scales a lane holds of a tile: row lane % 16
     uint4 w[DEPTH][SL][2];
-    float s[DEPTH][NS];
-    uint32_t z[DEPTH][ZEROS ? NS : 1];
+    uint32_t s[DEPTH][NS], z[DEPTH][ZEROS ? NS : 1];  // their bits
+    float b[DEPTH][2];                                // biases of rows g and g + 8 (one warp a tile)
     // the cursor: the item to be loaded next
     int b0 = 0, lap = 0, i = 0;
     const uint8_t *p, *p8;     // rows g and g + 8 of its first tile at this lane's first byte
-    int rows, left;            // rows and bytes of k left from there on
+    int n0, rows, left;        // its first row; rows and bytes of k left from there on
     bool full;                 // all there, in whole vectors: the loads need no checks
     int64_t sp;                // where this lane's row of scales begins
     int group0;                // and its group
 
     __device__ __forceinline__ void aim(const Q4Args &a, const Place &at) {
-        const int list = b0 + i, n0 = at.row(a, list, at.r_warp), first = at.c_lo + (lap * a.wk + at.k_warp) * SL;
+        const int list = b0 + i, first = at.c_lo + (lap * a.wk + at.k_warp) * SL;
         const int byte = first * 64 + at.t * 16;
+        n0 = at.row(a, list, at.r_warp);
         rows = list < at.lists && first < at.c_hi ? a.n - n0 : 0;
         left = (a.k + 1) / 2 - byte;
         full = a.w_vec && rows >= a.depth * 16 && (first + SL) * 64 <= (a.k + 1) / 2;
@@ -233,13 +257,20 @@ struct Stream {
 #pragma unroll
         for (int x = 0; x < NS; x++) {
             const int group = int((uint64_t(uint32_t(group0 + 2 * x)) * a.per_mul) >> 31);
-            s[d][x] = 0.0f;
+            s[d][x] = 0;
             if constexpr (ZEROS) z[d][x] = 8;
             if (there && (NG > 1 || at.lane < 16) && group < a.groups) {
                 const int64_t q = sp + int64_t(d) * 16 * a.groups + group;
-                s[d][x] = load_scale(a, q);
-                if constexpr (ZEROS) z[d][x] = uint32_t(__ldg(a.zeros + q)) & 15u;
+                s[d][x] = scale_bits(a, q);
+                if constexpr (ZEROS) z[d][x] = __ldg(a.zeros + q);
             }
+        }
+    }
+    __device__ __forceinline__ void biases(const Q4Args &a, const Place &at, int d) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = d * 16 + at.g + 8 * h;
+            b[d][h] = a.direct && a.bias && rows > r ? __ldg(a.bias + n0 + r) : 0.0f;
         }
     }
     __device__ __forceinline__ void next(const Q4Args &a, const Place &at) {
@@ -256,15 +287,16 @@ struct Stream {
 #pragma unroll
             for (int c = 0; c < SL; c++) chunk(a, at, d, c);
             scales(a, at, d);
+            biases(a, at, d);
         }
         next(a, at);
     }
     // group j's scale (zero point) of tile row r, in every lane
-    __device__ __forceinline__ float scale(int d, int j, int r) const {
-        return __shfl_sync(0xffffffffu, s[d][j >> 1], r | ((j & 1) << 4));
+    __device__ __forceinline__ float scale(const Q4Args &a, int d, int j, int r) const {
+        return scale_of(a, __shfl_sync(0xffffffffu, s[d][j >> 1], r | ((j & 1) << 4)));
     }
     __device__ __forceinline__ uint32_t zero(int d, int j, int r) const {
-        if constexpr (ZEROS) return __shfl_sync(0xffffffffu, z[d][j >> 1], r | ((j & 1) << 4));
+        if constexpr (ZEROS) return __shfl_sync(0xffffffffu, z[d][j >> 1], r | ((j & 1) << 4)) & 15u;
         return 8;
     }
 };
@@ -289,9 +321,8 @@ __device__ __forceinline__ void transpose(uint4 &u, int t) {
     u = make_uint4(a0, a1, a2, a3);
 }
 
-// One output value: the bias and the type.
+// One output value in its type.
 __device__ __forceinline__ void put_y(const Q4Args &a, int m, int n, float y) {
-    if (a.bias) y += __ldg(a.bias + n);
     const int64_t at = int64_t(m) * a.y_row + n;
     if (a.y_type == PPOCR_F32)
         static_cast<float *>(a.y)[at] = y;
@@ -301,41 +332,56 @@ __device__ __forceinline__ void put_y(const Q4Args &a, int m, int n, float y) {
         static_cast<__nv_bfloat16 *>(a.y)[at] = __float2bfloat16_rn(y);
 }
 
-// The join of `count` lists from `list0` on: value(list of the batch, tile of
-// the list, row of x, row of the tile) adds up the block's warps, the
-// cluster's blocks follow, finish(m, n, y) takes the sum.
+__device__ __forceinline__ void peer_store(float *p, uint32_t rank, float v) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+
+// The join of `count` lists from `list0` on, in pieces of 32 values (a tile's 16
+// rows for two rows of x): value(list of the batch, tile of the list, row of
+// x, row of the tile) adds up the block's warps; in a cluster piece p goes to
+// block p mod ks, which adds the blocks' in rank order; finish(m, n, y, bias,
+// scale) takes the sum.
 template <class V, class F>
-__device__ __forceinline__ void join(const Q4Args &a, const Place &at, int rows, int list0, int count, float *part, const V &value,
-                                     const F &finish) {
+__device__ __forceinline__ void join(const Q4Args &a, const Place &at, int m0, int rows, int list0, int count, float *part,
+                                     const V &value, const F &finish) {
     __syncthreads();
-    const int per = 16 * rows, each = at.wr * a.depth, all = count * each * per;
-    const auto row_of = [&](int e) { return at.row(a, list0 + e / per / each, 0) + e / per % each * 16 + (e & 15); };
-    for (int e = threadIdx.x; e < all; e += blockDim.x) {
-        const int in = e % per, l = e / per;
-        const float y = value(l / each, l % each, in >> 4, in & 15);
+    const int each = at.wr * a.depth, pieces = (rows + 1) / 2, all = count * each * pieces, warps = int(blockDim.x) / 32;
+    const int r = at.lane & 15, mine = (all + a.ks - 1) / a.ks;
+    const auto end = [&](int p, float y) {
+        const int tile = p / pieces, m = (p - tile * pieces) * 2 + (at.lane >> 4);
+        const int n = at.row(a, list0 + tile / each, 0) + tile % each * 16 + r;
+        if (m >= rows || n >= a.n) return;
+        finish(m, n, y, a.bias ? __ldg(a.bias + n) : 0.0f, a.x_groups == 1 ? __ldg(a.x_scales + m0 + m) : 1.0f);
+    };
+    for (int p = at.warp; p < all; p += warps) {
+        const int tile = p / pieces, m = (p - tile * pieces) * 2 + (at.lane >> 4);
+        const float y = m < rows ? value(tile / each, tile % each, m, r) : 0.0f;
         if (a.ks > 1)
-            part[e] = y;
-        else if (row_of(e) < a.n)
-            finish(in >> 4, row_of(e), y);
+            peer_store(part + (at.rank * mine + p / a.ks) * 32 + at.lane, uint32_t(p % a.ks), y);
+        else
+            end(p, y);
     }
-    if (a.ks > 1) {
-        cluster_sync();
-        for (int e = at.rank * int(blockDim.x) + threadIdx.x; e < all; e += a.ks * int(blockDim.x)) {
-            float y = 0.0f;
-            for (int x = 0; x < a.ks; x++) y += peer_load(part + e, uint32_t(x));
-            if (row_of(e) < a.n) finish(e % per >> 4, row_of(e), y);
-        }
-        cluster_sync();
-    } else {
+    if (a.ks == 1) {
         __syncthreads();
+        return;
     }
+    cluster_sync();
+    for (int q = at.warp; q * a.ks + at.rank < all; q += warps) {
+        float y = 0.0f;
+        for (int x = 0; x < a.ks; x++) y += part[(x * mine + q) * 32 + at.lane];
+        end(q * a.ks + at.rank, y);
+    }
+    if (list0 + count < at.lists) cluster_sync();  // the next batch's pieces come to the same place
 }
 
 // Splits the work and launches: blocks of up to `warps` warps, items of up to
 // `depth` tiles by `sl` chunks, `cols` partial sums a tile row and warp,
-// `stage` bytes of shared memory a warp besides.
+// `stage` bytes of shared memory a warp besides, `direct` where a warp alone can
+// write its tiles' results.
 cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth, int bpg, int cols, int stage, int shared_most,
-                      cudaStream_t stream) {
+                      bool direct, cudaStream_t stream) {
     const int passes = (a.m + a.cols_rows - 1) / a.cols_rows, sms = sm_count();
     a.chunks = (a.k + 127) / 128;
     const uint32_t per = uint32_t(a.group) / (32 * bpg);
@@ -360,10 +406,11 @@ cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth
     const int wr = warps / a.wk, lists = (items + wr - 1) / wr;
     int teams = sms / a.ks;
     teams = lists < teams ? lists : teams;
-    const int list_floats = warps * depth * 16 * cols, part_floats = a.ks > 1 ? wr * depth * 16 * a.cols_rows : 0;
+    const int list_floats = warps * depth * 16 * cols, part_floats = a.ks > 1 ? wr * depth * (a.cols_rows + 1) / 2 * 32 + a.ks * 32 : 0;
     const int fit = (shared_most - warps * stage) / 4 / (list_floats + part_floats), mine = (lists + teams - 1) / teams;
     a.batch = fit < mine ? fit : mine;
     a.red_floats = a.batch * list_floats;
+    a.direct = direct && a.wk == 1 && a.ks == 1 && a.laps == 1;
     a.stage_floats = a.batch * (list_floats + part_floats);
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(unsigned(teams * a.ks), unsigned(passes));
