@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
             if (a.laps > 1 || b0 == 0) load(c0);
             for (int i = 0; i < count; i++) {
                 in.aim(a, at);
+                const bool more = in.rows > 0;  // there is another item to take
 #pragma unroll
                 for (int d = 0; d < DEPTH; d++) {
                     if (d >= a.depth) break;
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                             s[j / (4 / BPG)][j % (4 / BPG)][h] = in.scale(a, d, j, at.g + 8 * h) * Enter<XT>::SCALE;
                             z[j / (4 / BPG)][j % (4 / BPG)][h] = in.zero(d, j, at.g + 8 * h);
                         }
-                    in.scales(a, at, d);
+                    if (more) in.scales(a, at, d);
 #pragma unroll
                     for (int c = 0; c < SL; c++) {
                         uint4 u0 = in.w[d][c][0], u1 = in.w[d][c][1];
@@ -216,10 +217,10 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
                                 }
                             }
                         }
-                        in.chunk(a, at, d, c);
+                        if (more) in.chunk(a, at, d, c);
                     }
                     const float bias[2] = {in.b[d][0], in.b[d][1]};
-                    in.biases(a, at, d);
+                    if (more) in.biases(a, at, d);
                     if (PARTS == 1 && a.direct) {
                         // this warp's sums are whole: out with them
                         const int n0 = at.row(a, b0 + i, at.r_warp) + d * 16 + at.g;

@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
             if (a.laps > 1 || b0 == 0) load(at.c_lo + (lap * a.wk + at.k_warp) * SL);
             for (int i = 0; i < count; i++) {
                 in.aim(a, at);
+                const bool more = in.rows > 0;  // there is another item to take
 #pragma unroll
                 for (int d = 0; d < DEPTH; d++) {
                     if (d >= a.depth) break;
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                             s[j][h] = in.scale(a, d, j, at.g + 8 * h);
                             z[j][h] = in.zero(d, j, at.g + 8 * h);
                         }
-                    in.scales(a, at, d);
+                    if (more) in.scales(a, at, d);
 #pragma unroll
                     for (int c = 0; c < SL; c++) {
                         uint4 u0 = in.w[d][c][0], u1 = in.w[d][c][1];
@@ -197,10 +198,10 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
                                 acc[3] = fmaf(__int_as_float(v[3]) - 12582912.0f, s[j][1], acc[3]);
                             }
                         }
-                        in.chunk(a, at, d, c);
+                        if (more) in.chunk(a, at, d, c);
                     }
                     const float bias[2] = {in.b[d][0], in.b[d][1]};
-                    in.biases(a, at, d);
+                    if (more) in.biases(a, at, d);
                     // columns 2t and 2t + 1 are bytes 0, 1 (t even) or 2, 3 of a row: one number
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
