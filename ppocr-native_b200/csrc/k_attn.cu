@@ -212,6 +212,8 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     if (overlap(out, on, q, qn) || (s->kv_rows && (overlap(out, on, k, kn) || overlap(out, on, v, vn))))
         return refuse(PPOCR_E_ARG, me, "out overlaps q, k or v");
 
+    if (const int bad = check_buffers(me, {q, s->kv_rows ? k : nullptr, s->kv_rows ? v : nullptr, out, q_offsets, k_begin, k_len})) return bad;
+
     AttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.out = out;
     a.q_offsets = q_offsets, a.k_begin = k_begin, a.k_len = k_len;

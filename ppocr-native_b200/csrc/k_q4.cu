@@ -326,6 +326,7 @@ extern "C" int ppocr_matvec_q4(const ppocr_matvec_q4_shape *s, const void *x, co
         (bias && overlap(y, yn, bias, s->n * uint64_t(4))) ||
         (x_scales && overlap(y, yn, x_scales, s->rows * (s->x_group ? groups : 1) * 4)))
         return refuse(PPOCR_E_ARG, me, "y overlaps another buffer");
+    if (const int bad = check_buffers(me, {x, x_scales, w, scales, zeros, bias, y})) return bad;
     a.scale_type = s->scale_type, a.y_type = s->y_type;
     // one group in all is the row's scale
     a.x_groups = !x_scales ? 0 : s->x_group ? int(groups) : 1;

@@ -383,6 +383,7 @@ extern "C" int ppocr_rms_norm_e4m3(const ppocr_rms_norm_shape *s, const void *x,
         overlap(y, yn, x, xn) || overlap(y, yn, residual, rn) || overlap(y, yn, gamma, gn) || overlap(y, yn, scales, cn) ||
         overlap(scales, cn, x, xn) || overlap(scales, cn, residual, rn) || overlap(scales, cn, gamma, gn))
         return refuse(PPOCR_E_ARG, me, "an output overlaps another buffer");
+    if (const int bad = check_buffers(me, {x, residual, gamma, sum, y, scales})) return bad;
     const auto wide = [&](const void *p, int64_t row) { return !p || (aligned(p, 16) && uint64_t(row) * size % 16 == 0); };
     const bool vec = c % 8 == 0 && aligned(gamma, 16) && wide(x, a.x_row) && wide(residual, a.r_row) && wide(sum, a.sum_row) && aligned(y, 8) && a.y_row % 8 == 0;
     const auto str = static_cast<cudaStream_t>(stream);

@@ -202,6 +202,40 @@ def test_attention_lowest_scores(cuda_mod, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [40, 128])
+@pytest.mark.parametrize("steps", [False, True])
+def test_attention_maxima_that_grow(cuda_mod, t, d, steps):
+    # keys whose scores rise along the lane, far past the last maximum tile by
+    # tile, and fall again: the running sums are rescaled both ways
+    lens = [(2, 900), (1, 700)] if steps else [(700, 700), (130, 130)]
+    a = Attn(t, lens, 4, 2, d, 400, 30, 5, seed=11, interleaved=False, room=901)
+    rise = torch.linspace(0, 6, a.k.shape[0] // 2, device="cuda")
+    a.k.mul_(torch.cat([rise, rise.flip(0)])[:, None, None].to(a.k.dtype))
+    a.call()
+    a.check()
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,left,right,sinks", [(128, 700, 0, 4), (64, -1, -1, 0), (80, 300, 300, 130)])
+def test_attention_one_long_lane(cuda_mod, t, d, left, right, sinks):
+    a = Attn(t, [(2300, 2300)], 4, 2, d, left, right, sinks, seed=12, pad=1)
+    a.call()
+    a.check()
+
+
+@gpu
+def test_attention_many_lanes_of_steps(cuda_mod):
+    # more lanes than are sorted by length, and fewer, empty ones among them
+    for lanes in (300, 200):
+        lens = [(1, 1 + (i * 37) % 210) if i % 9 else (0, 5) for i in range(lanes)]
+        a = Attn("bf16", lens, 8, 2, 64, 100, 0, 2, seed=13, room=211, pad=2)
+        a.call()
+        a.check()
+
+
+@gpu
 def test_attention_hints_size_the_launch_only(cuda_mod):
     a = Attn("bf16", [(300, 300), (9, 9), (150, 150)], 4, 2, 64, 64, 0, 2, seed=7)
     for hint in ((1, 1), (0, 0), (10 ** 6, 10 ** 6), (20, 300)):
@@ -415,7 +449,8 @@ class Q4:
 @pytest.mark.parametrize("m,k,n,group", [(1, 1, 1, 32), (1, 120, 360, 32), (2, 64, 17, 64), (3, 1000, 777, 32),
                                          (5, 257, 100, 128), (8, 4096, 64, 128), (9, 640, 130, 64), (16, 1024, 48, 128),
                                          (17, 333, 50, 96), (32, 2049, 40, 32), (1, 8192, 300, 128), (1, 40000, 33, 256),
-                                         (31, 5000, 20, 64), (1, 100, 40000, 32)])
+                                         (31, 5000, 20, 64), (1, 100, 40000, 32), (16, 4096, 20000, 64),
+                                         (2, 2048, 9000, 32), (20, 20000, 70, 128), (9, 70000, 40, 64), (2, 70000, 20, 128)])
 def test_q4(cuda_mod, xt, zeros, m, k, n, group):
     for yt in ("f32", "bf16", "f16"):
         # rows on 16 bytes and rows side by side
@@ -463,6 +498,26 @@ def test_q4_rows_of_x_are_apart(cuda_mod, xt):
         a.value = a.x.double()
         a.call()
         a.check()
+
+
+@gpu
+def test_buffers_elsewhere_are_refused(cuda_mod):
+    # plain host memory would fault on the device: refused before any launch
+    host = torch.zeros(4096, dtype=torch.float32)
+    buffers = [torch.zeros(4096, dtype=torch.float32, device="cuda") for _ in range(9)]
+    dev = [b.data_ptr() for b in buffers]
+    calls = {
+        "attention": lambda p: cuda.attention_window(cuda.AttentionShape("f32", 1, 1, 1, 8, 4, 4, 1.0), *p[:7]),
+        "norm": lambda p: cuda.rms_norm_e4m3(cuda.RmsNormShape("f32", 4, 8), *p[:6]),
+        "q4": lambda p: cuda.matvec_q4(cuda.MatvecQ4Shape("f32", "f32", "f32", 2, 32, 4, 32), p[0], None, *p[1:6]),
+    }
+    for name, call in calls.items():
+        for i in range(7 if name == "attention" else 6):
+            p = list(dev)
+            p[i] = host.data_ptr()
+            with pytest.raises(cuda.PpocrError) as e:
+                call(p)
+            assert e.value.code == cuda.E_ARG and "device memory" in str(e.value), (name, i, str(e.value))
 
 
 # ---------------------------------------------------------------- together
