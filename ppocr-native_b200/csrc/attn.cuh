@@ -147,13 +147,14 @@ struct TileOf {
 // f16 and bf16: m16n8k16 with f32 accumulation; the probabilities are
 // rounded to the type for the second product (2^-9 or 2^-12 of each, the
 // size of the output's own rounding), the sum l keeps them unrounded.
-// f32: each product as three tf32 ones (hi*hi + hi*lo + lo*hi).
+// f32: each product as three tf32 ones (hi*hi + hi*lo + lo*hi), the sums of a tile
+// apart from those of the lane.
 template <class T, int DP>
 struct WarpAttn {
     static constexpr int STRIDE = TileOf<T, DP>::STRIDE;
     static constexpr int ND = DP / 8;
     float o[ND][4];
-    float m[2], l[2];
+    float m[2], l[2], keep[2];
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -185,8 +186,12 @@ struct WarpAttn {
         } else {
             const int g = lane >> 2, t = lane & 3;
             const uint32_t qa = qs + uint32_t((g * STRIDE + t) * 4), ka = ks + uint32_t((g * STRIDE + t) * 4);
-            // unrolled by two only: the f32 form is bound by its own matrix
-            // instructions, and more would spill
+            // The matrix units cut a sum's low bits where f32 addition rounds them, always
+            // toward zero: the small products go into sums of their own.
+            float small[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) small[n][0] = small[n][1] = small[n][2] = small[n][3] = 0.0f;
+            // unrolled by two only: more would spill
 #pragma unroll 2
             for (int kk = 0; kk < DP / 8; kk++) {
                 uint32_t qh[4], ql[4];
@@ -199,11 +204,15 @@ struct WarpAttn {
                     uint32_t h0, h1, l0, l1;
                     split_tf32(lds(ka + uint32_t(n * 8 * STRIDE * 4) + kk * 32), h0, l0);
                     split_tf32(lds(ka + uint32_t(n * 8 * STRIDE * 4) + kk * 32 + 16), h1, l1);
-                    mma8_tf32(s[n], ql, h0, h1);
-                    mma8_tf32(s[n], qh, l0, l1);
+                    mma8_tf32(small[n], ql, h0, h1);
+                    mma8_tf32(small[n], qh, l0, l1);
                     mma8_tf32(s[n], qh, h0, h1);
                 }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[n][e] += small[n][e];
         }
     }
 
@@ -222,7 +231,7 @@ struct WarpAttn {
             top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
             top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
         }
-        float from[2], keep[2];
+        float from[2];
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -242,7 +251,8 @@ struct WarpAttn {
             }
         l[0] = fmaf(l[0], keep[0], sum[0]);
         l[1] = fmaf(l[1], keep[1], sum[1]);
-        if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+        // (f32's sums take the factor as they take the tile)
+        if (sizeof(T) == 2 && __any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < ND; n++) {
                 o[n][0] *= keep[0];
@@ -275,22 +285,29 @@ struct WarpAttn {
             // 2t + 1, where this lane's probabilities are
             const int g = lane >> 2, t = lane & 3;
             const uint32_t va = vs + uint32_t((2 * t * STRIDE + g) * 4);
+            uint32_t ph[NT][4], pl[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                uint32_t ph[4], pl[4];
-                split_tf32(s[n][0], ph[0], pl[0]);
-                split_tf32(s[n][2], ph[1], pl[1]);
-                split_tf32(s[n][1], ph[2], pl[2]);
-                split_tf32(s[n][3], ph[3], pl[3]);
+                split_tf32(s[n][0], ph[n][0], pl[n][0]);
+                split_tf32(s[n][2], ph[n][1], pl[n][1]);
+                split_tf32(s[n][1], ph[n][2], pl[n][2]);
+                split_tf32(s[n][3], ph[n][3], pl[n][3]);
+            }
+            // the tile's sums by themselves, then into o by a rounded addition
 #pragma unroll
-                for (int c = 0; c < ND; c++) {
+            for (int c = 0; c < ND; c++) {
+                float sum[4] = {}, small[4] = {};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
                     uint32_t h0, h1, l0, l1;
                     split_tf32(lds(va + uint32_t((n * 8 * STRIDE + c * 8) * 4)), h0, l0);
                     split_tf32(lds(va + uint32_t(((n * 8 + 1) * STRIDE + c * 8) * 4)), h1, l1);
-                    mma8_tf32(o[c], pl, h0, h1);
-                    mma8_tf32(o[c], ph, l0, l1);
-                    mma8_tf32(o[c], ph, h0, h1);
+                    mma8_tf32(small, pl[n], h0, h1);
+                    mma8_tf32(small, ph[n], l0, l1);
+                    mma8_tf32(sum, ph[n], h0, h1);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[c][e] = fmaf(o[c][e], keep[e >> 1], sum[e] + small[e]);
             }
         }
     }

@@ -217,11 +217,13 @@ __device__ __forceinline__ void mma8_tf32(float c[4], const uint32_t a[4], uint3
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// An f32 value as two tf32 ones, each rounded to nearest: hi*hi + hi*lo + lo*hi
-// leaves out 2^-24 of a product and what 2^-23 of it the low half rounds away.
+// An f32 value as its tf32 neighbour (in whole-number steps: rounded to nearest,
+// 19.6 us on the page lines' attention where cvt.rna took 23.2) and the exact
+// remainder, of which the matrix instruction reads 11 bits: hi*hi + hi*lo + lo*hi
+// loses about 2^-22 of a product. An infinity's remainder is NaN.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
 }  // namespace
