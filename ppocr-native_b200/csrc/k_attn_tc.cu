@@ -33,6 +33,7 @@ namespace {
 constexpr int BQ = 128, SOFTMAX_WARPS = 4, MMA_WARP = SOFTMAX_WARPS, COPY_WARP = SOFTMAX_WARPS + 1, THREADS = SOFTMAX_WARPS * 32 + 64;
 constexpr int BOX = 32;                    // rows a copy brings: 4 KB of one 64-column panel
 constexpr int BOX_BYTES = BOX * 128;
+constexpr unsigned long long DRAIN_NS = 200ull * 1000 * 1000;
 constexpr float GROW = 8.0f;               // log2 of how far a maximum may grow before O is rescaled
 
 struct Maps {
@@ -284,11 +285,19 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                 if (tl.n > 1) load_k(1);
                 load_v(0);
                 if (tl.n > 1) load_v(1);
+                int k_end = min(tl.n, 2), v_end = k_end;
                 for (int it = 2; it < tl.n; it++) {
                     if (!__all_sync(0xffffffffu, wait(s_bar + buf(it) * 8, phase(it - 2)))) break;  // K is read
                     load_k(it);
+                    k_end = it + 1;
                     if (!__all_sync(0xffffffffu, wait(o_bar + buf(it) * 8, phase(it - 2)))) break;  // V is read
                     load_v(it);
+                    v_end = it + 1;
+                }
+                if (v_end < tl.n) {  // given up: not before the copies in flight have landed
+                    drain(q_bar, turn & 1, DRAIN_NS);
+                    for (int it = max(0, k_end - 2); it < k_end; it++) drain(k_bar + buf(it) * 8, phase(it), DRAIN_NS);
+                    for (int it = max(0, v_end - 2); it < v_end; it++) drain(v_bar + buf(it) * 8, phase(it), DRAIN_NS);
                 }
             }
             __syncwarp();
@@ -314,8 +323,12 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                     }
                 };
                 scores(0);
+                int s_end = on, o_end = 0;  // tiles whose products were issued
                 for (int it = 0; it < tl.n; it++) {
-                    if (it + 1 < tl.n) scores(it + 1);
+                    if (it + 1 < tl.n) {
+                        scores(it + 1);
+                        s_end += on;
+                    }
                     const int n = (tl.count(it) + 15) / 16;
                     on &= __all_sync(0xffffffffu, wait(v_bar + buf(it) * 8, phase(it)) && wait(p_bar + buf(it) * 8, phase(it)));
                     fence_after();
@@ -323,6 +336,11 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                         value_product(n, tmem + O_COL, tmem + buf(it) * BK, v_desc + buf(it) * next, id_o, it > 0);
                         commit(o_bar + buf(it) * 8);
                     }
+                    o_end += on;
+                }
+                if (!on) {  // given up: not before the products in flight are done
+                    if (s_end > 0) drain(s_bar + buf(s_end - 1) * 8, phase(s_end - 1), DRAIN_NS);
+                    if (o_end > 0) drain(o_bar + buf(o_end - 1) * 8, phase(o_end - 1), DRAIN_NS);
                 }
             }
             __syncwarp();
