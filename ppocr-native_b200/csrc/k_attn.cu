@@ -183,8 +183,8 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     if (!std::isfinite(s->scale) || s->scale < 0.0f) return refuse(PPOCR_E_ARG, me, "scale must be finite and not negative");
     if (!s->head_dim || s->head_dim > 128) return refuse(PPOCR_E_SIZE, me, "head_dim must be between 1 and 128");
     if (s->heads > 65535 || s->lanes > 65535) return refuse(PPOCR_E_SIZE, me, "more than 65535 heads or lanes");
-    const uint64_t most = uint64_t(1) << 40, rows_most = uint64_t(1) << 30;
-    if (s->q_rows > rows_most || s->kv_rows > rows_most) return refuse(PPOCR_E_SIZE, me, "more than 2^30 rows");
+    const uint64_t most = uint64_t(1) << 40, rows_most = uint64_t(1) << 29;
+    if (s->q_rows > rows_most || s->kv_rows > rows_most) return refuse(PPOCR_E_SIZE, me, "more than 2^29 rows");
     if (s->q_row > most || s->q_head > most || s->k_row > most || s->k_head > most || s->v_row > most ||
         s->v_head > most || s->out_row > most || s->out_head > most)
         return refuse(PPOCR_E_SIZE, me, "a stride above 2^40 elements");
@@ -201,7 +201,7 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     const bool apart = (s->out_head >= d || s->heads == 1) && (s->out_row >= uint64_t(s->heads - 1) * s->out_head + d || s->q_rows == 1);
     const bool apart2 = (s->out_row >= d || s->q_rows == 1) && (s->out_head >= (s->q_rows - 1) * s->out_row + d || s->heads == 1);
     if (!apart && !apart2) return refuse(PPOCR_E_ARG, me, "output rows or heads overlap");
-    // 2^30 rows x 2^40 elements fit neither the card nor 64 bits of bytes
+    // 2^29 rows x 2^40 elements fit neither the card nor 64 bits of bytes
     const auto span = [&](uint64_t rows, uint64_t row, uint64_t heads, uint64_t head) {
         const double n = (rows ? double(rows - 1) : 0.0) * double(row) + double(heads - 1) * double(head) + double(d);
         return n > 1e15 ? uint64_t(0) : rows ? ((rows - 1) * row + (heads - 1) * head + d) * size : uint64_t(1);
@@ -222,8 +222,8 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     a.v_row = int64_t(s->v_row), a.v_head = int64_t(s->v_head), a.out_row = int64_t(s->out_row), a.out_head = int64_t(s->out_head);
     a.lanes = int(s->lanes), a.heads = int(s->heads), a.kv_heads = int(s->kv_heads), a.share = a.heads / a.kv_heads;
     a.d = int(s->head_dim);
-    // positions lie below 2^30 in size, so these limits cut nothing and sums stay in 32 bits
-    const int32_t far = (int32_t(1) << 30) - 2;
+    // positions lie below 2^29 in size, so these limits cut nothing and sums stay in 32 bits
+    const int32_t far = int32_t(1) << 29;
     a.left = s->left, a.right = s->right < far ? s->right : far;
     a.left = a.left < far ? a.left : far;
     a.sinks = int(s->sinks < uint32_t(far) ? s->sinks : uint32_t(far));

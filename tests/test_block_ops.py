@@ -501,6 +501,62 @@ def test_q4_rows_of_x_are_apart(cuda_mod, xt):
 
 
 @gpu
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("m,k,n,group", [(1, 700, 90, 32), (2, 700, 90, 64), (2, 5000, 40, 128), (1, 33, 17, 32)])
+def test_q4_one_and_two_rows_with_no_numbers(cuda_mod, xt, m, k, n, group):
+    # whole-number sums have no infinity: such a row is done another way, the
+    # row beside it as before
+    a = Q4(xt, "f32", m, k, n, group, seed=4)
+    a.call()
+    a.check()
+    clean = a.y.clone()
+    x = a.x.float()
+    x[0, k // 2] = math.nan
+    a.x = x.to(a.x.dtype)
+    a.call()
+    assert bool(a.y[0].isnan().all()) and torch.equal(a.y[1:], clean[1:])
+    if xt != "e4m3":
+        x[0, k // 2] = -math.inf
+        a.x = x.to(a.x.dtype)
+        a.call()
+        assert not bool(a.y[0].isfinite().any()) and torch.equal(a.y[1:], clean[1:])
+        # magnitudes far apart: the largest decides the step, 2^-31 of it
+        tiny = torch.finfo(torch.float32).tiny if xt != "f16" else 2.0 ** -14
+        x = a.value.float() * tiny
+        a.x = x.to(a.x.dtype)
+        a.value = a.x.double()
+        a.bias.zero_()
+        a.scales.fill_(1.0)
+        a.call()
+        q = torch.stack([a.w & 15, a.w >> 4], 2).flatten(1)[:, :k].double()
+        w = q - a.zeros.double()[:, torch.arange(k, device="cuda") // group]
+        off = (a.y.double() - a.value @ w.T).abs()
+        assert bool((off <= (a.value.abs() @ w.T.abs()) * (k + 16) * 2.0 ** -23 + 2.0 ** -149 * k).all())
+
+
+@gpu
+def test_first_calls_inside_a_capture(cuda_mod, tmp_path):
+    # a fresh process whose first call of each operator is a captured one
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    here = Path(__file__).resolve().parent
+    code = (f"import sys; sys.path.insert(0, {str(here)!r})\n"
+            "import conftest, torch\n"
+            "from test_block_ops import block_buffers, block_step\n"
+            "dev = block_buffers(20); x = torch.randn(20, 128, device='cuda').half(); start = dev['res'].clone()\n"
+            "g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n"
+            "    block_step(dev, x, 20)\n"
+            "g.replay(); torch.cuda.synchronize(); got = dev['res'].clone(); dev['res'].copy_(start)\n"
+            "block_step(dev, x, 20); torch.cuda.synchronize()\n"
+            "assert torch.equal(got, dev['res']) and bool(got.isfinite().all())\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@gpu
 def test_buffers_elsewhere_are_refused(cuda_mod):
     # plain host memory would fault on the device: refused before any launch
     host = torch.zeros(4096, dtype=torch.float32)
