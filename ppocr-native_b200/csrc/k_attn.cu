@@ -242,8 +242,23 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
         keys = keys < seen ? keys : seen;
     }
     const auto str = static_cast<cudaStream_t>(stream);
-    // few query rows a key head (single steps): the keys are split instead
-    if (uint64_t(max_q) * a.share <= 16) {
+    // The split form walks a tile's keys with 4 to 32 warps and takes the heads that
+    // share a key head as rows of one tile; the others walk them alone, 64 or 128
+    // queries of a head at a time. Split, then,
+    // - where its tiles fill the card at most once and there are keys to split (8 key
+    //   heads of 64, window 1024, a query: 7.6 us where the others take 20 in bf16 and 79
+    //   in f32; 17 keys: 5.8 us, 4.7 and 5.9; 16 lanes of 16 queries: 15, 28 and 80 us);
+    // - where its tiles are half as many as the others' blocks or fewer (32 lanes of
+    //   4 heads a key head: 27 us, 63 and 358);
+    // - in f32 with keys to split, unless they are more (32 lanes of 16 queries: 48 us and
+    //   112; of 64: 182 and 119). Beyond, bf16 at head size 64 and 128: 27 and 35 us
+    //   for 32 lanes of one query and head where the others take 30 and 29.
+    const bool f32 = s->type == PPOCR_F32;
+    const uint64_t sms = uint64_t(sm_count()), per_head = uint64_t(a.lanes) * a.kv_heads;
+    const uint64_t tiles = (uint64_t(max_q) * a.share + 15) / 16 * per_head;
+    const uint64_t blocks = (uint64_t(max_q) + 63) / 64 * a.share * per_head;
+    if ((tiles <= sms && keys >= (f32 ? 64 : 256)) || (2 * tiles <= blocks && blocks > sms) ||
+        (f32 && tiles <= blocks && keys >= 256)) {
         const cudaError_t e = launch_attn_split(a, s->type, max_q, uint32_t(keys), str);
         return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
     }

@@ -267,7 +267,7 @@ cudaError_t start_split(AttnArgs a, uint32_t max_q, uint32_t max_keys, cudaStrea
     const uint64_t alone = tiles * a.lanes * a.kv_heads;
     // blocks a tile: until the card is full or every warp has one key tile
     uint32_t blocks = 1;
-    while (blocks < MOST_BLOCKS && alone * blocks < uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
+    while (blocks < MOST_BLOCKS && alone * blocks * 2 <= uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
     a.sort = alone * blocks > uint64_t(sm_count()) && a.lanes > 1 && a.lanes <= SORT_LANES;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(unsigned(tiles * blocks), unsigned(a.kv_heads), unsigned(a.lanes));

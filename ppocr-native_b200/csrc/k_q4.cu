@@ -260,7 +260,7 @@ cudaError_t start(Q4Args a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     a.cols_rows = Q::COLS / Enter<XT>::PARTS < a.m ? Q::COLS / Enter<XT>::PARTS : a.m;
     return launch_q4(reinterpret_cast<const void *>(q4_kernel<XT, CT, BPG, ZEROS>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, Q::WIDE, 0,
-                     Q::SHARED, Enter<XT>::PARTS == 1, stream);
+                     Q::SHARED, Enter<XT>::PARTS == 1, Enter<XT>::PARTS == 1, stream);
 }
 
 template <class XT, int BPG, bool ZEROS>
@@ -333,7 +333,12 @@ extern "C" int ppocr_matvec_q4(const ppocr_matvec_q4_shape *s, const void *x, co
     a.w_vec = aligned(w, 16) && a.w_row % 16 == 0;
     a.x_vec = uint64_t(a.x_row) * xs % (xs == 1 ? 8 : 16) == 0 && aligned(x, xs == 1 ? 8 : 16);
     const auto str = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = a.m <= 2                  ? launch_q4_int(a, s->x_type, str)
+    // one or two rows in whole numbers: f32 always (k 120 to 8192: 5.3 to 53 us where
+    // three parts take 9.8 to 157), the others from 2^25 weights on (bf16, groups of
+    // 128 without zero points, 4096 x 4096: 7.1 us, 6.7 the other way; 8192 x 8192:
+    // 13.3 and 16.0; 28672 x 8192: 28 and 40)
+    const bool whole = a.m <= 2 && (s->x_type == PPOCR_F32 || s->n * uint64_t(s->k) >= uint64_t(1) << 25);
+    const cudaError_t e = whole                     ? launch_q4_int(a, s->x_type, str)
                           : s->x_type == PPOCR_F32  ? start_x<float>(a, str)
                           : s->x_type == PPOCR_F16  ? start_x<__half>(a, str)
                           : s->x_type == PPOCR_BF16 ? start_x<__nv_bfloat16>(a, str)

@@ -233,7 +233,7 @@ cudaError_t start(Q4Args a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     a.cols_rows = a.m;
     return launch_q4(reinterpret_cast<const void *>(q4_int_kernel<XT, BPG, ZEROS, ROWS_X>), a, Q::WARPS, Q::SL, Q::DEPTH, BPG, ROWS_X,
-                     Q::SL * 4 * 4 * ROWS_X * 32, Q::SHARED, true, stream);
+                     Q::SL * 4 * 4 * ROWS_X * 32, Q::SHARED, true, false, stream);
 }
 
 template <class XT, int BPG>

@@ -379,19 +379,23 @@ __device__ __forceinline__ void join(const Q4Args &a, const Place &at, int m0, i
 // Splits the work and launches: blocks of up to `warps` warps, items of up to
 // `depth` tiles by `sl` chunks, `cols` partial sums a tile row and warp,
 // `stage` bytes of shared memory a warp besides, `direct` where a warp alone can
-// write its tiles' results.
+// write its tiles' results, `laps` where laps cost little.
 cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth, int bpg, int cols, int stage, int shared_most,
-                      bool direct, cudaStream_t stream) {
+                      bool direct, bool laps, cudaStream_t stream) {
     const int passes = (a.m + a.cols_rows - 1) / a.cols_rows, sms = sm_count();
     a.chunks = (a.k + 127) / 128;
     const uint32_t per = uint32_t(a.group) / (32 * bpg);
     a.per_mul = ((1u << 31) + per - 1) / per;
-    // k over one block's warps, then over a cluster's blocks, then in laps
+    // k over one block's warps, then over a cluster's blocks, then in laps; where a
+    // slice of x comes in as it is (`laps`), in laps before a cluster's join holds up
+    // more tiles than there are SMs (16 rows f16 or bf16, k 16384: n 256 in clusters
+    // 11.8 us, in laps 22.5; n 2048 28.4 and 22.8; 32 rows, k 8192, n 4096 65 and 38;
+    // f32, whose slices are taken apart each lap, 66 and 240, 137 and 258, 186 and 295)
     const int slices = (a.chunks + sl - 1) / sl;
     a.wk = 1;
     while (a.wk < warps && a.wk < slices) a.wk *= 2;
     a.ks = 1;
-    while (a.ks < 8 && a.ks * a.wk < slices) a.ks *= 2;
+    while (a.ks < 8 && a.ks * a.wk < slices && (!laps || int64_t((a.n + 15) / 16) * passes * a.ks * 2 <= sms)) a.ks *= 2;
     a.share = (slices + a.ks - 1) / a.ks * sl;
     a.laps = (a.share + a.wk * sl - 1) / (a.wk * sl);
     // fewer tiles an item, then fewer items a block, as long as every item still

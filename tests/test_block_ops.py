@@ -236,6 +236,35 @@ def test_attention_many_lanes_of_steps(cuda_mod):
 
 
 @gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [16, 40, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (2, 2), (12, 1)])
+@pytest.mark.parametrize("left,right,sinks", [(-1, -1, 0), (400, 3, 9), (-1, 0, 0), (290, 0, 40)])
+def test_attention_some_queries_over_many_keys(cuda_mod, t, d, heads, kv_heads, left, right, sinks):
+    # tiles of 16 rows that hold several queries and heads, the last one short
+    lens = [(33, 700), (5, 300), (20, 20), (0, 50), (40, 10), (1, 900), (16, 33)]
+    a = Attn(t, lens, heads, kv_heads, d, left, right, sinks, seed=21, room=903, pad=4)
+    a.call()
+    a.check()
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [20, 64, 120])
+def test_attention_many_short_lanes(cuda_mod, t, d):
+    # heads that share a key head in one tile, keys too few to split
+    lens = [(1 + i % 3, 1 + (i * 7) % 60) if i % 11 else (0, 5) for i in range(60)]
+    a = Attn(t, lens, 16, 2, d, 40, 0, 3, seed=22, room=61, pad=2)
+    a.call()
+    a.check()
+    # one head a key head, more tiles than SMs
+    lens = [(16 - i % 4, 300 + 13 * i) for i in range(20)]
+    a = Attn(t, lens, 8, 8, d, 350, 0, 1, seed=23, room=560, pad=1)
+    a.call()
+    a.check()
+
+
+@gpu
 def test_attention_hints_size_the_launch_only(cuda_mod):
     a = Attn("bf16", [(300, 300), (9, 9), (150, 150)], 4, 2, 64, 64, 0, 2, seed=7)
     for hint in ((1, 1), (0, 0), (10 ** 6, 10 ** 6), (20, 300)):
@@ -532,6 +561,22 @@ def test_q4_one_and_two_rows_with_no_numbers(cuda_mod, xt, m, k, n, group):
         w = q - a.zeros.double()[:, torch.arange(k, device="cuda") // group]
         off = (a.y.double() - a.value @ w.T).abs()
         assert bool((off <= (a.value.abs() @ w.T.abs()) * (k + 16) * 2.0 ** -23 + 2.0 ** -149 * k).all())
+
+
+@gpu
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("m,group,zeros", [(1, 128, False), (2, 128, True), (2, 64, True), (1, 32, True)])
+def test_q4_large_products_of_one_and_two_rows(cuda_mod, xt, m, group, zeros):
+    # odd sizes beyond 2^25 weights
+    a = Q4(xt, "f32", m, 4129, 8203, group, zeros=zeros, seed=9)
+    a.call()
+    a.check()
+    clean = a.y.clone()
+    x = a.x.float()
+    x[0, 2001] = math.nan
+    a.x = x.to(a.x.dtype)
+    a.call()
+    assert bool(a.y[0].isnan().all()) and torch.equal(a.y[1:], clean[1:])
 
 
 @gpu
