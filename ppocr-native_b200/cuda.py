@@ -348,7 +348,15 @@ def db_mask(prob: int, pixels: int, thresh: float, mask: int, stream: int | None
 TYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}
 
 
-class AttentionShape(ctypes.Structure):
+class _Shape(ctypes.Structure):
+    """A call's sizes; `ref`, its address, is taken once and again by a copy."""
+
+    def __setstate__(self, *state):
+        super().__setstate__(*state)
+        self.ref = ctypes.addressof(self)
+
+
+class AttentionShape(_Shape):
     """`ppocr_attention_shape`: a layer's sizes, kept by the caller across
     calls. Types by name ("f32", "f16", "bf16"); strides as (row, head) pairs
     in elements, None for rows of `heads` x `head_dim` elements side by side;
@@ -372,7 +380,7 @@ class AttentionShape(ctypes.Structure):
         self.ref = ctypes.addressof(self)
 
 
-class RmsNormShape(ctypes.Structure):
+class RmsNormShape(_Shape):
     """`ppocr_rms_norm_shape`; strides in elements, 0 for rows side by side."""
 
     _fields_ = [("type", ctypes.c_int32), ("channels", ctypes.c_uint32), ("group", ctypes.c_uint32),
@@ -385,7 +393,7 @@ class RmsNormShape(ctypes.Structure):
         self.ref = ctypes.addressof(self)
 
 
-class MatvecQ4Shape(ctypes.Structure):
+class MatvecQ4Shape(_Shape):
     """`ppocr_matvec_q4_shape`; x_row and y_row in elements, w_row in bytes, 0
     for rows side by side."""
 

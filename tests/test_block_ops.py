@@ -379,6 +379,22 @@ def test_norm(cuda_mod, t, group, rows, c):
 
 @gpu
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [0, 64])
+@pytest.mark.parametrize("rows,c", [(9001, 100), (4001, 500), (2600, 1001), (2600, 1024), (1300, 2047), (1301, 4096), (700, 5003),
+                                    (700, 8192)])
+def test_norm_more_rows_than_blocks(cuda_mod, t, group, rows, c):
+    g = torch.Generator("cuda").manual_seed(c)
+    x, r = (torch.randn(rows, c, generator=g, device="cuda").to(DTYPES[t]) for _ in range(2))
+    gamma = torch.randn(c, generator=g, device="cuda")
+    s, y = torch.empty_like(x), torch.empty(rows, c, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(rows, -(-c // group) if group else 1, device="cuda")
+    cuda.rms_norm_e4m3(cuda.RmsNormShape(t, rows, c, group, 1e-5), x.data_ptr(), r.data_ptr(), gamma.data_ptr(),
+                       s.data_ptr(), y.data_ptr(), scales.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    norm_check(t, x, r, gamma, 1e-5, group, s, y, scales)
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("c,row", [(120, 121), (264, 272), (100, 104), (1000, 1003)])
 def test_norm_strides_and_in_place(cuda_mod, t, c, row):
     rows = 37
@@ -577,6 +593,16 @@ def test_q4_large_products_of_one_and_two_rows(cuda_mod, xt, m, group, zeros):
     a.x = x.to(a.x.dtype)
     a.call()
     assert bool(a.y[0].isnan().all()) and torch.equal(a.y[1:], clean[1:])
+
+
+@gpu
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("m,k,n,group", [(3, 9000, 2500, 64), (9, 4200, 2400, 32), (20, 5003, 1200, 128), (32, 8192, 4100, 96)])
+def test_q4_many_tiles_of_long_rows(cuda_mod, xt, m, k, n, group):
+    # more tiles than SMs and more k than a block's warps hold at once
+    a = Q4(xt, "f32", m, k, n, group, seed=17)
+    a.call()
+    a.check()
 
 
 @gpu
@@ -824,6 +850,17 @@ def test_q4_refuses(code, kw):
         q4_call(**kw)
     assert e.value.code == code, str(e.value)
     assert "ppocr_matvec_q4" in str(e.value)
+
+
+def test_copied_shapes_stand_alone():
+    import copy
+    import pickle
+
+    a = cuda.AttentionShape(type="f32", lanes=1, heads=2, kv_heads=2, head_dim=8, q_rows=3, kv_rows=3, scale=1.0)
+    for b in (copy.copy(a), copy.deepcopy(a), pickle.loads(pickle.dumps(a))):
+        assert b.ref == ctypes.addressof(b) != a.ref and bytes(b) == bytes(a)
+        b.lanes = 7
+        assert a.lanes == 1 and cuda.AttentionShape.from_address(b.ref).lanes == 7
 
 
 def test_empty_calls_do_nothing():
