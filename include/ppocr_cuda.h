@@ -205,8 +205,8 @@ typedef struct {
     int32_t left, right;                     /* keys seen before and behind the query's own; -1: no limit */
     uint32_t sinks;                          /* a lane's first keys, seen however far back they are */
     float scale;                             /* of the scores, not negative */
-    uint32_t max_q, max_k;                   /* about the longest lane's queries and keys (0: unknown); they size
-                                                the launch, never the result */
+    uint32_t max_q, max_k;                   /* about the longest lane's queries and keys (0: unknown); they choose
+                                                the launch, never more than a rounding of the result */
     uint64_t q_rows, kv_rows;                /* rows q and out, and k and v, hold (at most 2^29) */
     uint64_t q_row, q_head, k_row, k_head;   /* strides from row to row and head to head */
     uint64_t v_row, v_head, out_row, out_head;
@@ -271,9 +271,10 @@ typedef struct {
  * ceil(k / 2) bytes or more; ceil(k / group) scales and zero points (a byte each, 0 to 15; NULL:
  * 8) a row; bias f32 or NULL. e4m3 rows of x (ppocr_rms_norm_e4m3's) come with
  * their x_scales. Products are exact and sums f32 (f32 rows of x as three bf16
- * parts); one and two rows of x enter as whole numbers of 2^-31 of the largest
- * of each 256 or 512 k, and their sums are exact but for the scales. Scales
- * below 2^112; a row of x with an infinity or NaN spoils that row of y alone.
+ * parts); one and two rows of f32, or of any type times 2^25 weights or more,
+ * enter as whole numbers of 2^-31 of the largest of each 256 or 512 k, and their
+ * sums are exact but for the scales. Scales below 2^112; a row of x with an
+ * infinity or NaN spoils that row of y alone.
  * y is rounded once. Fastest with w and w_row multiples of 16 bytes. y overlaps nothing else. */
 int ppocr_matvec_q4(const ppocr_matvec_q4_shape *shape, const void *x, const float *x_scales, const uint8_t *w,
                     const void *scales, const uint8_t *zeros, const float *bias, void *y, void *stream);

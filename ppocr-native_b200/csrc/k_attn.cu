@@ -6,9 +6,13 @@
 // the key tiles they see (sinks, then the window), 64 keys a tile, two
 // buffers filled by cp.async while the other is used (32 in f32, whose
 // products are three each: a finer step leaves less of a narrow window's tiles
-// hidden); tiles outside every query's window are never read, those outside a
-// warp's are skipped, tiles inside every window skip the masks. Bound by the
-// warp-level matrix instructions.
+// hidden, and more blocks an SM; 2000 queries of 8 heads of 128, window 256: 72
+// us, 103 with 64); tiles outside every query's window are never read, those
+// outside a warp's are skipped, tiles inside every window skip the masks.
+//
+// Bound by the issue of instructions: f32 takes three products a pair and the
+// splitting of their operands. 44 lines of 10 to 200 queries, 8 heads of 15 in
+// f32, window 49: 20 us (8.4 MB, 1.3 us of HBM; 10.6 M warp instructions).
 #include <cmath>
 
 #include "attn.cuh"
@@ -250,15 +254,17 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     //   in f32; 17 keys: 5.8 us, 4.7 and 5.9; 16 lanes of 16 queries: 15, 28 and 80 us);
     // - where its tiles are half as many as the others' blocks or fewer (32 lanes of
     //   4 heads a key head: 27 us, 63 and 358);
-    // - in f32 with keys to split, unless they are more (32 lanes of 16 queries: 48 us and
-    //   112; of 64: 182 and 119). Beyond, bf16 at head size 64 and 128: 27 and 35 us
-    //   for 32 lanes of one query and head where the others take 30 and 29.
+    // - in f32 with keys to split, up to twice as many tiles as blocks or SMs (32 lanes
+    //   of 32 queries, head sizes 16, 64 and 128: 30, 93 and 238 us, 48, 116 and 216
+    //   the other way; of 64 queries: 50, 182 and 415 and 49, 119 and 223).
+    // Beyond, in bf16, head sizes 64 and 128: 27 and 35 us for 32 lanes of one query
+    // and head where the others take 30 and 29.
     const bool f32 = s->type == PPOCR_F32;
     const uint64_t sms = uint64_t(sm_count()), per_head = uint64_t(a.lanes) * a.kv_heads;
     const uint64_t tiles = (uint64_t(max_q) * a.share + 15) / 16 * per_head;
     const uint64_t blocks = (uint64_t(max_q) + 63) / 64 * a.share * per_head;
     if ((tiles <= sms && keys >= (f32 ? 64 : 256)) || (2 * tiles <= blocks && blocks > sms) ||
-        (f32 && tiles <= blocks && keys >= 256)) {
+        (f32 && tiles <= 2 * (blocks > sms ? blocks : sms) && keys >= 256)) {
         const cudaError_t e = launch_attn_split(a, s->type, max_q, uint32_t(keys), str);
         return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
     }

@@ -8,7 +8,10 @@
 // states become one in its shared memory, with weights 2^(m_i - max m), and the
 // cluster's meet through distributed shared memory: row r is joined by block
 // r mod cluster. No workspace, nothing to clear.
-// Bound by the keys' and values' bytes; a single lane by latency.
+// Bound by the keys' and values' bytes; a single lane by latency. 64 lanes of
+// one query behind 300 to 12 000 keys, 32 heads over 8 of 128, window 4096, bf16:
+// 155 us, 919 MB at 5.9 TB/s (0.9 of a plain copy's rate). One lane, 516 keys, 16
+// heads over 4 of 64: 6.4 us, of which an empty launch is 2.2.
 #include "attn.cuh"
 
 namespace ppocr {
@@ -265,7 +268,9 @@ cudaError_t start_split(AttnArgs a, uint32_t max_q, uint32_t max_keys, cudaStrea
     if (e != cudaSuccess) return e;
     const uint64_t rows = uint64_t(max_q) * a.share, tiles = rows ? (rows + 15) / 16 : 1;
     const uint64_t alone = tiles * a.lanes * a.kv_heads;
-    // blocks a tile: until the card is full or every warp has one key tile
+    // blocks a tile: while all clusters run at once and every warp has a key tile
+    // (4 lanes of one query and 8 key heads of 64, window 1024: 9.2 us with 4, 22.5
+    // with 8 blocks, which are more than the SMs)
     uint32_t blocks = 1;
     while (blocks < MOST_BLOCKS && alone * blocks * 2 <= uint64_t(sm_count()) && uint64_t(blocks) * WARPS * R::BK < max_keys) blocks *= 2;
     a.sort = alone * blocks > uint64_t(sm_count()) && a.lanes > 1 && a.lanes <= SORT_LANES;

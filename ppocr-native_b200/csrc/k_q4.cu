@@ -6,7 +6,9 @@
 // as they are, e4m3 as f16, f32 as three bf16 columns (8 bits of the mantissa
 // each) whose sums are added at the end. Bound by the unpacking of the
 // weights (11 instructions a word of 8) and, past 16 columns, by the matrix
-// instructions.
+// instructions; small products by latency. 16 rows f16, 120 x 18 710, groups of
+// 32: 4.9 us (2.6 MB, 0.4 us of HBM; an empty launch 2.2); 16 rows e4m3, 4096 x
+// 4096, groups of 64: 11.6 us (9.4 MB, 1.4 us).
 #include <type_traits>
 
 #include "q4.cuh"

@@ -9,6 +9,10 @@
 // x, before the f32 scale. What the fixed point drops of an x is at most
 // 2^-31 of its slice's largest, less than f32 sums round away. A slice with an
 // infinity or NaN gives NaN, and such results are done again the plain way.
+// Bound by HBM and, with zero points or small groups, by the groups' sums: one
+// row bf16, 8192 x 28 672, groups of 128: 25 to 28 us, 121 MB at 4.3 to 4.8 TB/s
+// (18.6 us at a plain copy's rate, the rest launch, x and join); groups of 64
+// with zero points 54 us, of 32 80 us.
 #include <type_traits>
 
 #include "q4.cuh"

@@ -399,7 +399,8 @@ cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth
     a.share = (slices + a.ks - 1) / a.ks * sl;
     a.laps = (a.share + a.wk * sl - 1) / (a.wk * sl);
     // fewer tiles an item, then fewer items a block, as long as every item still
-    // has a warp, and every block an SM, at once
+    // has a warp, and every block an SM, at once (16 rows, 120 x 18 710: 4.9 us, 9.6
+    // with items as they are, 5.6 with blocks as they are; 120 x 360: 4.5, 5.9, 5.7)
     const int64_t room = int64_t(sms) * (warps / a.wk) / (passes * a.ks);
     const auto items_of = [&](int d) { return (a.n + d * 16 - 1) / (d * 16); };
     while (depth > 1 && items_of(depth / 2) <= room) depth /= 2;
@@ -414,6 +415,7 @@ cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth
     const int fit = (shared_most - warps * stage) / 4 / (list_floats + part_floats), mine = (lists + teams - 1) / teams;
     a.batch = fit < mine ? fit : mine;
     a.red_floats = a.batch * list_floats;
+    // whole sums leave at once (16 rows, 120 x 18 710: 4.9 us, through the join 10.8)
     a.direct = direct && a.wk == 1 && a.ks == 1 && a.laps == 1;
     a.stage_floats = a.batch * (list_floats + part_floats);
     cudaLaunchConfig_t c{};
