@@ -315,7 +315,9 @@ struct WarpAttn {
 
 // One output row the plain way, by a whole warp, in f32 and over the keys it
 // sees alone: for rows that came out infinite or NaN above, since there a
-// masked key's zero weight times an infinity or NaN in its values is NaN.
+// masked key's zero weight times an infinity or NaN in its values is NaN, and
+// values near the largest number overflow where the weights, not yet divided by
+// their sum, exceed one.
 template <class T>
 __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i, int h) {
     const int lane = threadIdx.x & 31, p = i + ln.nk - ln.nq, kvh = h / a.share;
@@ -323,8 +325,8 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
     const T *k = static_cast<const T *>(a.k) + ln.k0 * a.k_row + kvh * a.k_head;
     const T *v = static_cast<const T *>(a.v) + ln.k0 * a.v_row + kvh * a.v_head;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = -INFINITY, sum = 0.0f;
-    for (int pass = 0; pass < 2; pass++) {
-        const float from = top == -INFINITY ? 0.0f : top;
+    for (int pass = 0; pass < 3; pass++) {  // the maximum, the sum, the output
+        const float from = top == -INFINITY ? 0.0f : top, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int j = 0; j < ln.nk; j++) {
             if (!sees(a, p, j)) {
                 // behind the sinks: on to the window; past it: done
@@ -339,9 +341,10 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
             s *= a.scale_log2;
             if (pass == 0) {
                 top = (s != s || top != top) ? NAN : fmaxf(top, s);
+            } else if (pass == 1) {
+                sum += exp2_fast(s - from);
             } else {
-                const float w = exp2_fast(s - from);
-                sum += w;
+                const float w = exp2_fast(s - from) * inv;
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (lane + 32 * e < a.d) acc[e] = fmaf(w, to_f32(v[j * a.v_row + lane + 32 * e]), acc[e]);
@@ -351,7 +354,7 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
     T *out = static_cast<T *>(a.out) + (ln.q0 + i) * a.out_row + h * a.out_head;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (lane + 32 * e < a.d) out[lane + 32 * e] = from_f32<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+        if (lane + 32 * e < a.d) out[lane + 32 * e] = from_f32<T>(acc[e]);
 }
 
 }  // namespace

@@ -174,9 +174,9 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile i
 
 // 2^x for x up to 16 on the multiply-add pipe, two at a time: x = n + f with f in
 // [-1/2, 1/2], 2^f by a polynomial of degree 4 (minimax by Lawson's weights,
-// 2.6e-6 relative), n into the exponent. Below -125: 2^-125.
+// 2.6e-6 relative), n into the exponent. Below -125: 0, so that a hidden key
+// weighs nothing; NaN becomes the largest number, infinity in 16 bits.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-    x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
     const float round = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers, which its low bits then hold
     const float2 r = fadd2(x, make_float2(round, round));
     const float2 f = ffma2(fadd2(r, make_float2(-round, -round)), make_float2(-1.0f, -1.0f), x);
@@ -185,8 +185,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
     p = ffma2(p, f, both(0.240247443318367f));
     p = ffma2(p, f, both(0.6931217908859253f));
     p = ffma2(p, f, both(0.9999992847442627f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+    return make_float2(x.x < -125.0f ? 0.0f : __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                       x.y < -125.0f ? 0.0f : __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
 
 // Bits 0 to n - 1.
@@ -468,7 +468,6 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
             if (tl.n > 0) ok &= wait(o_bar + buf(tl.n - 1) * 8, phase(tl.n - 1));
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            if (m == -INFINITY) l = 0.0f;  // no key was seen (the polynomial makes 2^-125 of a hidden one)
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             bool bad = !ok || !(l < INFINITY);
             T *out = static_cast<T *>(a.out) + (ln.q0 + i0 + row) * a.out_row + h * a.out_head;

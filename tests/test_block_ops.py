@@ -190,6 +190,44 @@ def test_attention_masked_places_may_hold_anything(cuda_mod, t, steps, bad, d):
 
 @gpu
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("steps", [False, True])
+def test_attention_large_values_in_masked_places(cuda_mod, t, d, steps):
+    # a weight of nearly nothing would show here: hidden keys have none at all
+    lens = [(2, 600), (1, 77)] if steps else [(300, 300), (77, 77)]
+    a = Attn(t, lens, 16, 16, d, 50, 0, 3, seed=15, interleaved=False, room=650)
+    huge = 6e4 if t == "f16" else 3e38
+    a.v[100:116] = huge
+    a.v[400:420] = -huge
+    a.v[630:650] = huge
+    a.call()
+    a.check()
+    # far below the others' scores: a weight of nothing, seen or not
+    if not steps:
+        b = Attn(t, lens, 16, 16, d, 200, 0, 3, seed=16, interleaved=False, room=300)
+        b.q[..., 0], b.k[..., 0] = 16, 0
+        b.k[100:140, :, 0] = -16 * d ** 0.5
+        b.v[100:140] = huge
+        b.call()
+        got = b.out[150:300].float()
+        assert bool((got.abs() < 8).all())
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_keys_of_no_number(cuda_mod, t, d):
+    # at every place of a tile: all the rows that see it, and no other
+    for j in (96, 97, 98, 99, 102, 103, 111, 127, 128, 135):
+        a = Attn(t, [(300, 300)], 16, 16, d, 50, 0, 3, seed=j, interleaved=False)
+        a.k[j, :, d // 2] = math.nan
+        a.call()
+        a.check()
+        assert bool(a.out[j:j + 51].isnan().all()) and bool(a.out[:j].isfinite().all()) and bool(a.out[j + 51:].isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_attention_lowest_scores(cuda_mod, t):
     # scores at the type's lowest values: no sum of weights may vanish
     a = Attn(t, [(70, 70), (1, 70)], 2, 2, 64, 20, 0, 1, seed=6, interleaved=False, room=70, scale=1.0)
