@@ -172,23 +172,6 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, volatile i
     return false;
 }
 
-// 2^x for x up to 16 on the multiply-add pipe, two at a time: x = n + f with f in
-// [-1/2, 1/2], 2^f by a polynomial of degree 4 (minimax by Lawson's weights,
-// 2.6e-6 relative), n into the exponent. Below -125: 0, so that a hidden key
-// weighs nothing; NaN becomes the largest number, infinity in 16 bits.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const float round = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers, which its low bits then hold
-    const float2 r = fadd2(x, make_float2(round, round));
-    const float2 f = ffma2(fadd2(r, make_float2(-round, -round)), make_float2(-1.0f, -1.0f), x);
-    const auto both = [](float c) { return make_float2(c, c); };
-    float2 p = ffma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
-    p = ffma2(p, f, both(0.240247443318367f));
-    p = ffma2(p, f, both(0.6931217908859253f));
-    p = ffma2(p, f, both(0.9999992847442627f));
-    return make_float2(x.x < -125.0f ? 0.0f : __int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                       x.y < -125.0f ? 0.0f : __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
-}
-
 // Bits 0 to n - 1.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
@@ -454,9 +437,7 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
 #pragma unroll
                         for (int x = 0; x < 16; x++) {
                             float2 e = ffma2(make_float2(s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]), scale2, base2);
-                            // a quarter of the exponentials beside the special-function unit (with 32
-                            // keys a tile the instructions are scarcer: 36.9 us against 35.5)
-                            e = BK == 64 && x % 4 == 3 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                             sum[x & 1] = fadd2(sum[x & 1], e);
                             w[x] = pack2<T>(e.x, e.y);
                         }

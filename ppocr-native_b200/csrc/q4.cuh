@@ -157,13 +157,6 @@ __device__ __forceinline__ uint4 pairs_of(const uint4 &v) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_load(const float *p, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
 
 // 16 bytes of weights, each read once: past L1.
 __device__ __forceinline__ uint4 load_once(const uint8_t *p) {
