@@ -9,6 +9,8 @@
 // instructions; small products by latency. 16 rows f16, 120 x 18 710, groups of
 // 32: 4.9 us (2.6 MB, 0.4 us of HBM; an empty launch 2.2); 16 rows e4m3, 4096 x
 // 4096, groups of 64: 11.6 us (9.4 MB, 1.4 us).
+// Three rows of f32 and more cost most: 16 rows, 4096 x 1024, groups of 64: 21 us,
+// f16 6.5, for three columns a row and the taking apart of x in each warp.
 #include <type_traits>
 
 #include "q4.cuh"
@@ -121,23 +123,28 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
 #pragma unroll
         for (int c = 0; c < SL; c++)
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+            for (int u = 0; u < 4; u++) {
+                float v[PARTS == 1 ? 1 : CT][8] = {};
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
-                    const int col = ct * 8 + at.g, r = col / PARTS;
+                    const int r = (ct * 8 + at.g) / PARTS;
                     const bool there = r < rows && c0 + c < at.c_hi;
-                    if constexpr (PARTS == 1) {
+                    if constexpr (PARTS == 1)
                         xf[c][u][ct] = take_x<XT>(a, m0 + r, k_of(c, u), there);
-                    } else {
-                        float v[8] = {};
-                        if (there) load_x<XT>(a, m0 + r, k_of(c, u), v);
+                    else if (there)
+                        load_x<XT>(a, m0 + r, k_of(c, u), v[ct]);
+                }
+                if constexpr (PARTS > 1) {
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        const int part = (ct * 8 + at.g) % PARTS;
                         uint32_t p[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            p[i] = pack2<M>(part_of(v[i], col % PARTS), part_of(v[i + 4], col % PARTS));
+                        for (int i = 0; i < 4; i++) p[i] = pack2<M>(part_of(v[ct][i], part), part_of(v[ct][i + 4], part));
                         xf[c][u][ct] = make_uint4(p[0], p[1], p[2], p[3]);
                     }
                 }
+            }
         if constexpr (PARTS == 1) {
 #pragma unroll
             for (int c = 0; c < SL; c++)

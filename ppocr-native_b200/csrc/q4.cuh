@@ -383,7 +383,7 @@ cudaError_t launch_q4(const void *kernel, Q4Args a, int warps, int sl, int depth
     // slice of x comes in as it is (`laps`), in laps before a cluster's join holds up
     // more tiles than there are SMs (16 rows f16 or bf16, k 16384: n 256 in clusters
     // 11.8 us, in laps 22.5; n 2048 28.4 and 22.8; 32 rows, k 8192, n 4096 65 and 38;
-    // f32, whose slices are taken apart each lap, 66 and 240, 137 and 258, 186 and 295)
+    // f32, whose slices are taken apart each lap, 61 and 240, 129 and 258, 181 and 295)
     const int slices = (a.chunks + sl - 1) / sl;
     a.wk = 1;
     while (a.wk < warps && a.wk < slices) a.wk *= 2;
