@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(Q4Tile<CT>::WARPS * 32, 1) q4_kernel(const __g
     const Place at(a);
     const int warps = int(blockDim.x) / 32;
     const int m0 = blockIdx.y * a.cols_rows, rows = min(a.cols_rows, a.m - m0);
+    if (a.ks > 1) cluster_arrive();
     Stream<SL, DEPTH, BPG, ZEROS> in;
     in.begin(a, at);
     uint4 xf[SL][4][CT];

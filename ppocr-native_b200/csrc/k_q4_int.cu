@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(IntTile<BPG>::WARPS * 32, 1) q4_int_kernel(con
     extern __shared__ __align__(16) float red[];  // [list of the batch][tile of the item][warp][row of x][16], the cluster's sums, x's stage
     const Place at(a);
     const int warps = int(blockDim.x) / 32;
+    if (a.ks > 1) cluster_arrive();
     Stream<SL, DEPTH, BPG, ZEROS> in;
     in.begin(a, at);
 

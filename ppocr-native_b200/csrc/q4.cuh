@@ -154,6 +154,10 @@ __device__ __forceinline__ uint4 pairs_of(const uint4 &v) {
                       __byte_perm(u[1], u[3], 0x7632));
 }
 
+// This block has started: another's shared memory may be written once all blocks of the
+// cluster have said so (cluster_wait).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -335,7 +339,7 @@ __device__ __forceinline__ void peer_store(float *p, uint32_t rank, float v) {
 // rows for two rows of x): value(list of the batch, tile of the list, row of
 // x, row of the tile) adds up the block's warps; in a cluster piece p goes to
 // block p mod ks, which adds the blocks' in rank order; finish(m, n, y, bias,
-// scale) takes the sum.
+// scale) takes the sum. The kernel has called cluster_arrive() before its first load.
 template <class V, class F>
 __device__ __forceinline__ void join(const Q4Args &a, const Place &at, int m0, int rows, int list0, int count, float *part,
                                      const V &value, const F &finish) {
@@ -348,6 +352,7 @@ __device__ __forceinline__ void join(const Q4Args &a, const Place &at, int m0, i
         if (m >= rows || n >= a.n) return;
         finish(m, n, y, a.bias ? __ldg(a.bias + n) : 0.0f, a.x_groups == 1 ? __ldg(a.x_scales + m0 + m) : 1.0f);
     };
+    if (a.ks > 1 && list0 == 0) cluster_wait();  // every block has started: its shared memory is there
     for (int p = at.warp; p < all; p += warps) {
         const int tile = p / pieces, m = (p - tile * pieces) * 2 + (at.lane >> 4);
         const float y = m < rows ? value(tile / each, tile % each, m, r) : 0.0f;
