@@ -271,9 +271,10 @@ typedef struct {
  * ceil(k / 2) bytes or more; ceil(k / group) scales and zero points (a byte each, 0 to 15; NULL:
  * 8) a row; bias f32 or NULL. e4m3 rows of x (ppocr_rms_norm_e4m3's) come with
  * their x_scales. Products are exact and sums f32 (f32 rows of x as three bf16
- * parts); one and two rows of f32, or of any type times 2^25 weights or more,
- * enter as whole numbers of 2^-31 of the largest of each 256 or 512 k, and their
- * sums are exact but for the scales. Scales below 2^112; a row of x with an
+ * parts). One and two rows of f32, and one row of another type times 2^26 weights or
+ * more, enter as whole numbers: x, with its scale, to 2^-62 of the largest of each
+ * 256 or 512 k (f32 exact down to 2^-38 of it, bf16 to 2^-54, f16 always), and their
+ * sums over 32 to 128 k are exact. Scales below 2^112; a row of x with an
  * infinity or NaN spoils that row of y alone.
  * y is rounded once. Fastest with w and w_row multiples of 16 bytes. y overlaps nothing else. */
 int ppocr_matvec_q4(const ppocr_matvec_q4_shape *shape, const void *x, const float *x_scales, const uint8_t *w,

@@ -1,5 +1,5 @@
 // ppocr_matvec_q4: a few rows of x times a matrix of 4-bit weights, and its
-// form for three rows and more (one and two: k_q4_int.cu).
+// form for three rows and more, and for fewer where k_q4_int.cu is no faster.
 //
 // A weight becomes q - z, a small integer that f16 and bf16 hold exactly; its
 // scale multiplies each group's f32 sum. x enters exactly too: f16 and bf16
@@ -343,11 +343,12 @@ extern "C" int ppocr_matvec_q4(const ppocr_matvec_q4_shape *s, const void *x, co
     a.w_vec = aligned(w, 16) && a.w_row % 16 == 0;
     a.x_vec = uint64_t(a.x_row) * xs % (xs == 1 ? 8 : 16) == 0 && aligned(x, xs == 1 ? 8 : 16);
     const auto str = static_cast<cudaStream_t>(stream);
-    // one or two rows in whole numbers: f32 always (k 120 to 8192: 5.3 to 53 us where
-    // three parts take 9.8 to 157), the others from 2^25 weights on (bf16, groups of
-    // 128 without zero points, 4096 x 4096: 7.1 us, 6.7 the other way; 8192 x 8192:
-    // 13.3 and 16.0; 28672 x 8192: 28 and 40)
-    const bool whole = a.m <= 2 && (s->x_type == PPOCR_F32 || s->n * uint64_t(s->k) >= uint64_t(1) << 25);
+    // in whole numbers: one or two rows of f32 (two rows, groups of 128, 4096 x 4096 and 8192 x
+    // 28 672: 9.4 and 41 us; one row 7.8 and 27, where three parts take 157), and one row of
+    // another type from 2^26 weights on (bf16, 8192 x 4096, 8192 and 28 672, groups of 128
+    // without zero points: 9.4, 13.4 and 27 us, 9.3, 16.0 and 40 the other way; groups of 64
+    // with them: 13.4, 22.5 and 56, 12.1, 22.7 and 61; two rows 18 and 16, 40 and 40)
+    const bool whole = s->x_type == PPOCR_F32 ? a.m <= 2 : a.m == 1 && s->n * uint64_t(s->k) >= uint64_t(1) << 26;
     const cudaError_t e = whole                     ? launch_q4_int(a, s->x_type, str)
                           : s->x_type == PPOCR_F32  ? start_x<float>(a, str)
                           : s->x_type == PPOCR_F16  ? start_x<__half>(a, str)

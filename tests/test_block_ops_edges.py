@@ -47,3 +47,117 @@ def test_q4_clusters_beside_other_work(cuda_mod, xt, m, k, n, group):
         a.y.zero_()
         a.call()
         assert torch.equal(a.y, want)
+
+
+def q4_close(a):
+    """As Q4.check for f32 outputs, with errors that add up as the root of their number.
+    S is the root of the sum of the products' squares; partial sums of terms of any sign
+    stay below 3 S or so. A group's sum takes at most 8 instructions of 16 k, each cutting at
+    most 2^-23 of it, all toward zero: 24 S 2^-23 over the groups, whose signs differ. Each of
+    the G groups' additions rounds 2^-24 of at most 3 S, independently: sqrt(G) S 2^-23. Eight
+    more roundings end it (joins, scales, the bias, a product of x and its scale)."""
+    _, _, _, m, k, n, group, _ = a.args
+    q = torch.stack([a.w & 15, a.w >> 4], 2).flatten(1)[:, :k].double()
+    each = torch.arange(k, device="cuda") // group
+    w = (q - (a.zeros.double()[:, each] if a.zeros is not None else 8)) * a.scales.double()[:, each]
+    want, squares = a.value @ w.T, a.value.square() @ w.T.square()
+    bias = a.bias.double() if a.bias is not None else torch.zeros(n, dtype=torch.float64, device="cuda")
+    tol = 2.0 ** -23 * (squares.sqrt() * (24 + math.sqrt(w.shape[1] / min(group, 128)) + 8) + (want + bias).abs())
+    off = (a.y.double() - want - bias).abs()
+    assert bool((off <= tol).all()), float((off / tol).nan_to_num(math.inf).max())
+    return tol
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,group", [(1, 120, 360, 32), (2, 64, 170, 64), (3, 1000, 777, 32), (5, 257, 100, 128),
+                                         (10, 4096, 64, 64), (11, 640, 130, 64), (32, 2049, 40, 32), (1, 8192, 300, 128),
+                                         (2, 8192, 300, 64), (4, 20000, 70, 128), (9, 9000, 40, 64)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_q4_f32_rows_keep_24_bits(cuda_mod, m, k, n, group, zeros):
+    a = Q4("f32", "f32", m, k, n, group, zeros, scale_type="f32", seed=k)
+    a.bias.zero_()
+    a.call()
+    tol = q4_close(a)
+    # the bound notices 16 bits in place of 24
+    cut = (a.x.view(torch.int32) & -256).view(torch.float32).double()
+    q = torch.stack([a.w & 15, a.w >> 4], 2).flatten(1)[:, :k].double()
+    each = torch.arange(k, device="cuda") // group
+    w = (q - (a.zeros.double()[:, each] if zeros else 8)) * a.scales.double()[:, each]
+    assert bool((((cut - a.value) @ w.T).abs() > tol).any())
+
+
+@gpu
+@pytest.mark.parametrize("xt,m,k,n", [("f32", 1, 512, 400), ("f32", 2, 512, 400), ("f32", 1, 5000, 90), ("f32", 2, 5000, 90),
+                                      ("f32", 3, 700, 90), ("f16", 1, 4129, 8203), ("bf16", 1, 4129, 8203),
+                                      ("f16", 2, 4129, 8203), ("bf16", 2, 4129, 8203), ("e4m3", 1, 4129, 8203),
+                                      ("f16", 1, 8257, 8203), ("bf16", 1, 8257, 8203), ("e4m3", 1, 8257, 8203)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("far", [10, 14, 20, 30])
+@pytest.mark.parametrize("hidden", ["weight", "scale"])
+def test_q4_one_value_far_above_the_rest(cuda_mod, xt, m, k, n, group, far, hidden):
+    # a channel that its weights take out again, by their zero point or their group's
+    # small scale: the others' sum keeps its bits
+    if xt in ("f16", "e4m3") and far > 10:
+        pytest.skip("beyond the type")
+    a = Q4(xt, "f32", m, k, n, group, True, scale_type="f32", seed=k + far)
+    a.bias.zero_()
+    x = a.x.float()
+    if xt == "e4m3":
+        x *= 2.0 ** -8
+        x[:, 77] = 256.0
+    else:
+        x[:, 77] = 1.7 * 2.0 ** far
+    a.x = x.to(a.x.dtype)
+    a.value = a.x.double() * (a.x_scales.double() if xt == "e4m3" else 1)
+    if hidden == "weight":
+        z = a.zeros[:, 77 // group]
+        a.w[:, 77 // 2] = (a.w[:, 77 // 2] & 15) | (z << 4)
+    else:
+        a.scales[:, 77 // group] = 2.0 ** -far * 2.0 ** -6
+    a.call()
+    q4_close(a)
+
+
+@gpu
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("group,zeros,x_group", [(128, False, 0), (128, True, 0), (64, True, 0), (32, True, 0), (96, False, 0),
+                                                 (64, True, 64)])
+def test_q4_one_row_of_very_many_weights(cuda_mod, xt, group, zeros, x_group):
+    # odd sizes beyond 2^26 weights, a NaN, and rows of w side by side
+    if x_group and xt != "e4m3":
+        pytest.skip("scales of x belong to e4m3")
+    for pad in (3, 0):
+        a = Q4(xt, "f32", 1, 8257, 8203, group, zeros, x_group=x_group, w_pad=pad, seed=19)
+        a.call()
+        a.check()
+        q4_close(a)
+        x = a.x.float()
+        x[0, 4001] = math.nan
+        a.x = x.to(a.x.dtype)
+        a.call()
+        assert bool(a.y.isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("k,group", [(300, 32), (5000, 128)])
+def test_q4_f32_rows_of_every_magnitude(cuda_mod, m, k, group):
+    # magnitudes spread over 2^39: what lies below 2^-62 of a slice's largest may go, no more
+    for top in (2.0 ** 100, 2.0 ** -110, 1.0):
+        a = Q4("f32", "f32", m, k, 70, group, scale_type="f32", seed=k)
+        a.bias.zero_()
+        a.x = torch.ldexp(a.x.clamp(-1, 1), torch.randint(-39, 1, a.x.shape, device="cuda")) * top
+        for hide in (False, True):
+            if hide:  # the largest taken out by its weight, the rest keep what they have
+                a.x[:, 40] = 3.0 * top
+                a.w[:, 20] = (a.w[:, 20] & 0xF0) | a.zeros[:, 40 // group]
+            a.value = a.x.double()
+            a.call()
+            q = torch.stack([a.w & 15, a.w >> 4], 2).flatten(1)[:, :k].double()
+            each = torch.arange(k, device="cuda") // group
+            w = (q - a.zeros.double()[:, each]) * a.scales.double()[:, each]
+            # q4_close's bound, and half a step of each x
+            want, squares = a.value @ w.T, a.value.square() @ w.T.square()
+            tol = 2.0 ** -23 * (squares.sqrt() * (32 + math.sqrt(k / min(group, 128))) + want.abs())
+            tol = tol + 3.0 * top * 2.0 ** -62 * w.abs().sum(1) + 2.0 ** -149 * k
+            assert bool(((a.y.double() - want).abs() <= tol).all())
