@@ -244,7 +244,8 @@ typedef struct {
 /* The residual's addition, a root-mean-square norm and its 8-bit output:
  *     s = x + residual,  n = s / sqrt(mean(s^2) + eps) * gamma,
  *     scale = max |n| over the group / 448,  y = e4m3(n / scale),
- * in f32 until the last rounding. s is written to `sum` rounded to the type
+ * in f32 until the last rounding (the squares' sum scaled where f32 does not hold it: s and
+ * s * gamma may be any f32 numbers). s is written to `sum` rounded to the type
  * (NULL: not written; x or residual themselves: updated in place) and
  * ceil(channels / group) scales a row to `scales`. residual may be NULL
  * (s = x). A group of zeros has scale 0 and zeros; one with a NaN, scale NaN and

@@ -8,7 +8,7 @@
 // four chunks a thread), so x and r are read once and nothing is read again: s
 // leaves rounded to the type, the norm uses the f32 s. The sum of squares is kept
 // in f32: lane sums, a shuffle tree, then the warps' sums in order (the same
-// order every time); the next row's loads are out while a row is worked on, and a
+// order every time), squares that leave its range in sums of scaled values; the next row's loads are out while a row is worked on, and a
 // row costs one barrier. Bound by HBM bytes: 16 384 rows of 4096 in bf16, groups
 // of 128: 80 us, 472 MB at 5.9 TB/s (0.9 of a plain copy's rate; 184 us without
 // the loads ahead). Rows that no vector width divides are read an element at a
@@ -127,6 +127,9 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// Factors that leave the squares of the largest f32 numbers, and of the least, in f32.
+constexpr float BIG = 0x1p-75f, TINY = 0x1p90f;
+
 // What the chunk's v = s * gamma are multiplied by for their 8 bits, from their
 // group's peak magnitude of n = v * inv: inv * 448 / peak. Where that quotient
 // leaves the quick division's range (or there is none: zeros, NaN), v becomes
@@ -151,11 +154,18 @@ __device__ __forceinline__ float steps_of(float peak, float inv, float v[8]) {
 // VEC: a chunk is 8 consecutive channels, 16-byte loads; else (rows, strides
 // or bases that 16 bytes do not divide) channels 32 apart, so that a warp's
 // loads lie side by side.
+//
+// Threads an SM: 1024 (64 registers), fewer where a thread holds two chunks and more.
 template <class T, int TPR, int CH, bool VEC>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const __grid_constant__ RmsArgs a) {
+constexpr int at_least = TPR == 1024 || CH == 1 ? 1024 / (TPR < 128 ? 128 : TPR)
+                                                : (!VEC ? 512 : sizeof(T) == 4 ? 768 : TPR == 32 ? 896 : 1024) / (TPR < 128 ? 128 : TPR);
+
+template <class T, int TPR, int CH, bool VEC>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, at_least<T, TPR, CH, VEC>) rms_norm_kernel(const __grid_constant__ RmsArgs a) {
     constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR, WARPS = TPR / 32;
     // two rows' in turn: between two writes of one lies the other's barrier
     __shared__ float part[2][WARPS], peak[2][WARPS];
+    __shared__ float3 wide[2][WARPS];  // where part is not a number
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = t / 32;
     const auto place = [&](int c) { return VEC ? (c * TPR + t) * 8 : (c * TPR + (t & ~31)) * 8 + lane; };
     const T *x = static_cast<const T *>(a.x), *r = static_cast<const T *>(a.r);
@@ -234,10 +244,44 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
                 }
             }
         }
-        fetch(row + int64_t(gridDim.x) * ROWS);
         float square = square2.x + square2.y;
+        // between 2^-80 and 2^100, or f32 may not hold this thread's squares (f16's lie between
+        // 2^-48 and 2^34): then they are taken again, of values times BIG or TINY, and square is
+        // not a number until the row's sum is made. Zeros have no squares to hold.
+        float3 apart = make_float3(0.0f, 0.0f, 0.0f);  // sums of squares as they are, times BIG^2, times TINY^2
+        const bool lost = place(0) < channels && __float_as_uint(square) - 0x17800000u >= 0x5A000000u;
+        const bool far = !std::is_same<T, __half>::value && __any_sync(0xffffffffu, lost);
+        if (far) {
+            const float by = square < 1.0f ? TINY : BIG;
+            float again = 0.0f;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+            for (int c = 0; c < CH; c++) {
+                if (!lost || place(c) >= channels) continue;
+                float x8[8], r8[8];
+                nx[c].get(x8);
+                if (r) nr[c].get(r8);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float w = (r ? x8[i] + r8[i] : x8[i]) * by;
+                    again = fmaf(w, w, again);
+                }
+            }
+            apart = make_float3(lost ? 0.0f : square, square < 1.0f ? 0.0f : again, square < 1.0f ? again : 0.0f);
+        }
+        fetch(row + int64_t(gridDim.x) * ROWS);
+        if (far) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) {
+                apart.x += __shfl_xor_sync(0xffffffffu, apart.x, d);
+                apart.y += __shfl_xor_sync(0xffffffffu, apart.y, d);
+                apart.z += __shfl_xor_sync(0xffffffffu, apart.z, d);
+            }
+            square = apart.y != 0.0f || apart.z != 0.0f ? NAN : apart.x;
+        } else {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) square += __shfl_xor_sync(0xffffffffu, square, d);
+            apart.x = square;
+        }
         float all = 0.0f;
         if (a.group == 0) {
 #pragma unroll
@@ -274,6 +318,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
         }
         if constexpr (WARPS > 1) {
             if (lane == 0) part[turn][warp] = square, peak[turn][warp] = all;
+            if (lane == 0 && square != square) wide[turn][warp] = apart;
             __syncthreads();
             square = 0.0f;
 #pragma unroll
@@ -282,9 +327,35 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
 #pragma unroll
                 for (int w = 0; w < WARPS; w++) all = peak2(all, peak[turn][w]);
             }
-            turn ^= 1;
         }
-        const float inv = rsqrtf(fmaf(square, a.inv_channels, a.eps));
+        // by: an exact factor that brings values far from one nearer
+        float mean = fmaf(square, a.inv_channels, a.eps), by = 1.0f;
+        if (!(mean > 0x1p-80f && mean < 0x1p100f)) {
+            // (a mean of zero or of no number goes through as it is)
+            if constexpr (WARPS > 1) {
+                // a warp's sums a lane: no loop here, which would end the wait for the loads in flight early
+                apart = make_float3(0.0f, 0.0f, 0.0f);
+                if (lane < WARPS) {
+                    apart.x = part[turn][lane];
+                    if (apart.x != apart.x) apart = wide[turn][lane];
+                }
+#pragma unroll
+                for (int d = 16; d; d >>= 1) {
+                    apart.x += __shfl_xor_sync(0xffffffffu, apart.x, d);
+                    apart.y += __shfl_xor_sync(0xffffffffu, apart.y, d);
+                    apart.z += __shfl_xor_sync(0xffffffffu, apart.z, d);
+                }
+            }
+            mean = fmaf(fmaf(apart.z * (1 / TINY), 1 / TINY, apart.x), a.inv_channels, a.eps);
+            if (apart.y != 0.0f) {
+                by = BIG, mean = fmaf(fmaf(apart.x * BIG, BIG, apart.y), a.inv_channels, a.eps * BIG * BIG);
+            } else if (mean < 0x1p-75f) {
+                by = TINY, mean = fmaf(apart.x * a.inv_channels * TINY, TINY, apart.z * a.inv_channels) + a.eps * TINY * TINY;
+            }
+        }
+        turn ^= 1;
+        const float inv = rsqrtf(mean);
+        all *= by;
         float *scales = a.scales + row * a.groups;
         uint8_t *y = a.y + row * a.y_row;
         if (a.group == 0 && channels && t == 0) scales[0] = all * inv * (1.0f / 448.0f);
@@ -292,8 +363,12 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
         for (int c = 0; c < CH; c++) {
             const int at = place(c), n = channels - at;
             if (n <= 0) continue;
+            if (by != 1.0f) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[c][i] *= by;
+            }
             if constexpr (VEC) {
-                const float p = (a.group ? top[c][0] : all) * inv;
+                const float p = (a.group ? top[c][0] * by : all) * inv;
                 if (a.group && (at & (a.group - 1)) == 0) scales[at >> a.group_log2] = p * (1.0f / 448.0f);
                 const float f = steps_of(p, inv, v[c]);
                 uint32_t w[2];
@@ -306,7 +381,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const _
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     if (i * 32 >= n) continue;
-                    const float p = (a.group ? top[c][i] : all) * inv;
+                    const float p = (a.group ? top[c][i] * by : all) * inv;
                     if (a.group && lane == 0 && ((at + i * 32) & (a.group - 1)) == 0) scales[(at + i * 32) >> a.group_log2] = p * (1.0f / 448.0f);
                     float one[8] = {v[c][i]};
                     const float f = steps_of(p, inv, one);

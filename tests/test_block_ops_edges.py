@@ -161,3 +161,51 @@ def test_q4_f32_rows_of_every_magnitude(cuda_mod, m, k, group):
             tol = 2.0 ** -23 * (squares.sqrt() * (32 + math.sqrt(k / min(group, 128))) + want.abs())
             tol = tol + 3.0 * top * 2.0 ** -62 * w.abs().sum(1) + 2.0 ** -149 * k
             assert bool(((a.y.double() - want).abs() <= tol).all())
+
+
+# ---------------------------------------------------------------- the norm
+
+def norm_run(t, x, r, gamma, eps, group):
+    rows, c = x.shape
+    s, y = torch.empty_like(x), torch.empty(rows, c, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(rows, -(-c // group) if group else 1, device="cuda")
+    cuda.rms_norm_e4m3(cuda.RmsNormShape(t, rows, c, group, eps), x.data_ptr(), r.data_ptr() if r is not None else None,
+                       gamma.data_ptr(), s.data_ptr(), y.data_ptr(), scales.data_ptr(),
+                       torch.cuda.current_stream().cuda_stream)
+    norm_check(t, x, r, gamma, eps, group, s, y, scales)
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [0, 64])
+@pytest.mark.parametrize("c", [100, 500, 1001, 1024, 2047, 4096, 8192, 20000, 32768])
+def test_norm_rows_far_from_one(cuda_mod, t, group, c):
+    # squares that f32 does not hold, alone or summed; rows of ordinary size among them
+    g = torch.Generator("cuda").manual_seed(c)
+    sizes = [1e18, 1.0, 1.8e19, 3e30, 1e38, 1e-15, 1e-19, 1e-23, 1e-30, 1e-35, 1.0, 6e-13, 3e-13, 1e-12, 2e-11, 1e15, 3e14, 1e16]
+    x = torch.randn(len(sizes), c, generator=g, device="cuda") * torch.tensor(sizes, device="cuda")[:, None]
+    x[0] = 1e18
+    x = x.clamp(-2e38, 2e38).to(DTYPES[t])
+    r = torch.zeros_like(x)
+    r[1] = 1
+    gamma = 0.5 + 0.5 * torch.rand(c, generator=g, device="cuda")
+    norm_run(t, x, r, gamma, 0.0, group)
+    norm_run(t, x, None, gamma, 0.0, group)
+    norm_run(t, x, r, gamma, 1e-6, group)
+    norm_run(t, x, r, gamma, 1e-37, group)
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("c", [120, 1003, 4096])
+def test_norm_rows_of_two_sizes(cuda_mod, t, c):
+    # one thread's channels far above, or below, all the others'; runs of zeros
+    g = torch.Generator("cuda").manual_seed(c)
+    for size in (1e25, 1e-25):
+        x = torch.randn(9, c, generator=g, device="cuda")
+        x[1:4, 40:48] *= size
+        x[4:6, 5] *= size
+        x[6:8] = 0
+        x[7:, 64:72] = size
+        norm_run(t, x.to(DTYPES[t]), None, torch.ones(c, device="cuda"), 1e-6, 0)
+        norm_run(t, x.to(DTYPES[t]), None, torch.ones(c, device="cuda"), 1e-6, 32)
