@@ -8,12 +8,13 @@
 // four chunks a thread), so x and r are read once and nothing is read again: s
 // leaves rounded to the type, the norm uses the f32 s. The sum of squares is kept
 // in f32: lane sums, a shuffle tree, then the warps' sums in order (the same
-// order every time), squares that leave its range in sums of scaled values; the next row's loads are out while a row is worked on, and a
-// row costs one barrier. Bound by HBM bytes: 16 384 rows of 4096 in bf16, groups
-// of 128: 80 us, 472 MB at 5.9 TB/s (0.9 of a plain copy's rate; 184 us without
-// the loads ahead). Rows that no vector width divides are read an element at a
-// time, 32 lanes side by side: 1009 rows of 1111 in f16 6.5 us (7.9 MB, 1.2 us
-// of HBM); 4096 channels so read would take 284 us.
+// order every time), squares that leave its range in sums of scaled values; the next
+// row's loads are out while a row is worked on, and a row costs one barrier. Bound
+// by HBM bytes: 16 384 rows of 4096 in bf16, groups of 128: 84 us, 472 MB at 5.6 TB/s
+// (0.86 of a plain copy's rate; 81 us without the test for squares out of range and
+// what follows it, 184 without the loads ahead). Rows that no vector width divides are
+// read an element at a time, 32 lanes side by side: 1009 rows of 1111 in f16 6.5 us
+// (7.9 MB, 1.2 us of HBM); 4096 channels so read would take 284 us.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -398,7 +399,7 @@ cudaError_t start(const RmsArgs &a, cudaStream_t stream) {
     static_assert(TPR == 32 || TPR >= 128, "a row is one warp's or a whole block's");
     constexpr int THREADS = TPR < 128 ? 128 : TPR, ROWS = THREADS / TPR;
     // all blocks at once where a thread has little to fetch ahead, else twice as many
-    // (bf16, 2048 channels: 79.3 us, 85.8 with twice as many; f32: 137 us, 164 with half)
+    // (bf16, 1024 channels: 42.6 us, 43.2 with twice as many; f32, 2048: 137 us, 164 with half)
     constexpr int AT_ONCE = sizeof(T) == 2 && CH == 1 && TPR > 32 ? 1024 : 2048;
     const int64_t want = (a.rows + ROWS - 1) / ROWS, most = int64_t(sm_count()) * (AT_ONCE / THREADS);
     rms_norm_kernel<T, TPR, CH, VEC><<<unsigned(want < most ? want : most), THREADS, 0, stream>>>(a);
@@ -421,7 +422,7 @@ cudaError_t start_c(const RmsArgs &a, cudaStream_t stream) {
     } else {
         // a chunk is 32 bytes: two a thread up to 4096 channels, then one as far as
         // threads go (f32, 2048 and 4096 channels: 137 and 141 us where one takes 141
-        // and 157; 8192: 154 us where two take 174)
+        // and 157; 8192: 154 us where two take 177)
         if (chunks <= 256) return start<T, 128, 2, VEC>(a, stream);
         if (chunks <= 512) return start<T, 256, 2, VEC>(a, stream);
         if (chunks <= 1024) return start<T, 1024, 1, VEC>(a, stream);
