@@ -61,6 +61,12 @@ __device__ __forceinline__ bool sees(const AttnArgs &a, int p, int j) {
     return (a.right < 0 || j <= p + a.right) && (a.left < 0 || j >= p - a.left || j < a.sinks);
 }
 
+// Whether position p sees any of nk keys.
+__device__ __forceinline__ bool sees_any(const AttnArgs &a, int p, int nk) {
+    const int hi = a.right < 0 ? nk : min(nk, p + a.right + 1), lo = a.left < 0 ? 0 : max(0, p - a.left);
+    return hi > 0 && (lo < hi || a.sinks > 0);
+}
+
 // The key tiles that queries at positions [p0, p1] need: the sinks below the
 // window first, then the window from a multiple of the tile size on.
 struct KeyTiles {
@@ -317,7 +323,9 @@ struct WarpAttn {
 // sees alone: for rows that came out infinite or NaN above, since there a
 // masked key's zero weight times an infinity or NaN in its values is NaN, and
 // values near the largest number overflow where the weights, not yet divided by
-// their sum, exceed one.
+// their sum, exceed one; and for rows that see keys whose weights all came out as
+// zeros, since a score above 0.69 of the largest number overflows in units of log2
+// (here the difference to the maximum is taken first, halved lest it overflow).
 template <class T>
 __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i, int h) {
     const int lane = threadIdx.x & 31, p = i + ln.nk - ln.nq, kvh = h / a.share;
@@ -326,7 +334,7 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
     const T *v = static_cast<const T *>(a.v) + ln.k0 * a.v_row + kvh * a.v_head;
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, top = -INFINITY, sum = 0.0f;
     for (int pass = 0; pass < 3; pass++) {  // the maximum, the sum, the output
-        const float from = top == -INFINITY ? 0.0f : top, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int j = 0; j < ln.nk; j++) {
             if (!sees(a, p, j)) {
                 // behind the sinks: on to the window; past it: done
@@ -338,13 +346,12 @@ __device__ __noinline__ void row_alone(const AttnArgs &a, const Lane &ln, int i,
             for (int c = lane; c < a.d; c += 32) s = fmaf(to_f32(q[c]), to_f32(k[j * a.k_row + c]), s);
 #pragma unroll
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            s *= a.scale_log2;
             if (pass == 0) {
                 top = (s != s || top != top) ? NAN : fmaxf(top, s);
             } else if (pass == 1) {
-                sum += exp2_fast(s - from);
+                sum += exp2_fast((0.5f * s - 0.5f * top) * (2.0f * a.scale_log2));
             } else {
-                const float w = exp2_fast(s - from) * inv;
+                const float w = exp2_fast((0.5f * s - 0.5f * top) * (2.0f * a.scale_log2)) * inv;
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (lane + 32 * e < a.d) acc[e] = fmaf(w, to_f32(v[j * a.v_row + lane + 32 * e]), acc[e]);

@@ -238,13 +238,13 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
                     if (x < blocks && lane + 32 * e < DP)
                         acc[e] = fmaf(m[x], peer_load(from[x] + uint32_t((r * DP + lane + 32 * e) * 4)), acc[e]);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            bool bad = false;
+            const int i = int((base + r) / a.share), h = kvh * a.share + int((base + r) % a.share);
+            bool bad = sum == 0.0f && sees_any(a, i + shift, ln.nk);
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 acc[e] *= inv;
                 bad |= !(fabsf(acc[e]) < INFINITY);
             }
-            const int i = int((base + r) / a.share), h = kvh * a.share + int((base + r) % a.share);
             if (__any_sync(0xffffffffu, bad)) {
                 row_alone<T>(a, ln, i, h);
             } else {

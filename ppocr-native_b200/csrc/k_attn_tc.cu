@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            bool bad = !ok || !(l < INFINITY);
+            bool bad = !ok || !(l < INFINITY) || (l == 0.0f && sees_any(a, p, ln.nk));
             T *out = static_cast<T *>(a.out) + (ln.q0 + i0 + row) * a.out_row + h * a.out_head;
             if (ok) {
                 for (int c = 0; c < dn; c += 16) {

@@ -209,3 +209,43 @@ def test_norm_rows_of_two_sizes(cuda_mod, t, c):
         x[7:, 64:72] = size
         norm_run(t, x.to(DTYPES[t]), None, torch.ones(c, device="cuda"), 1e-6, 0)
         norm_run(t, x.to(DTYPES[t]), None, torch.ones(c, device="cuda"), 1e-6, 32)
+
+
+# ---------------------------------------------------------------- attention
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("steps", [False, True])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_attention_scores_near_the_largest_number(cuda_mod, t, d, steps, sign):
+    # finite scores that their conversion to powers of two takes past the largest number:
+    # equal ones weigh the same, and one far above the others has all the weight
+    lens = [(2, 600), (1, 77)] if steps else [(300, 300), (77, 77)]
+    a = Attn(t, lens, 4, 2, d, 50, 0, 3, seed=41, interleaved=False, room=650, scale=1.0)
+    a.q.zero_(), a.k.zero_()
+    a.q[..., 0] = 1
+    a.k[..., 0] = sign * 3e38
+    a.call()
+
+    def weighted(weight):
+        # weight(j): a key's, by its place in the lane
+        at = 0
+        for (nq, nk), begin in zip(a.lens, a.begin):
+            p, j = torch.arange(nq, device="cuda")[:, None] + nk - nq, torch.arange(nk, device="cuda")[None]
+            seen = ((j <= p) & ((j >= p - 50) | (j < 3))).double() * weight(j)
+            v = a.v[begin:begin + nk].double().repeat_interleave(2, 1)
+            want = torch.einsum("ij,jhd->ihd", seen / seen.sum(1, keepdim=True), v)
+            mags = torch.einsum("ij,jhd->ihd", seen / seen.sum(1, keepdim=True), v.abs())
+            # weights (exact ones, their sum, a quotient) and the products' sum, then the output's rounding
+            tol = mags * (half_step(t) + (nk + 8) * 2.0 ** -23) + half_step(t) * want.abs()
+            assert bool(((a.out[at:at + nq].double() - want).abs() <= tol).all())
+            at += nq
+
+    weighted(lambda j: torch.ones_like(j).double())
+    # every seventh key above the rest by more than any weight holds
+    for begin, (_, nk) in zip(a.begin, a.lens):
+        j = torch.arange(nk, device="cuda")
+        a.k[begin:begin + nk, :, 0] = torch.where(j % 7 == 0, 3e38, 2.9e38 if sign > 0 else 3.2e38)[:, None].to(a.k.dtype) * sign
+    a.call()
+    weighted(lambda j: (j % 7 == 0).double())
