@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(ROW_THREADS, RowTile<T, DP>::BLOCKS) attn_rows
             }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
+            bad[r] = bad[r] && !no_numbers<T>(a, w.l[r]);
             const unsigned any = __ballot_sync(0xffffffffu, bad[r]);
             const int row = warp * 16 + r * 8 + (lane >> 2);
             bad[r] = (any >> (lane & 28)) & 15u;

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
                 acc[e] *= inv;
                 bad |= !(fabsf(acc[e]) < INFINITY);
             }
-            if (__any_sync(0xffffffffu, bad)) {
+            if (__any_sync(0xffffffffu, bad) && !no_numbers<T>(a, sum)) {
                 row_alone<T>(a, ln, i, h);
             } else {
                 T *out = static_cast<T *>(a.out) + (ln.q0 + i) * a.out_row + h * a.out_head;

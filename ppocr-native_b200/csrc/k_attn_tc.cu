@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
                 }
             }
             __syncwarp();
-            unsigned again = __ballot_sync(0xffffffffu, bad && row < rows);
+            unsigned again = __ballot_sync(0xffffffffu, bad && row < rows && !(ok && no_numbers<T>(a, l)));
             while (again) {
                 const int r = __ffs(again) - 1;
                 again &= again - 1;

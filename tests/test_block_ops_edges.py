@@ -249,3 +249,33 @@ def test_attention_scores_near_the_largest_number(cuda_mod, t, d, steps, sign):
         a.k[begin:begin + nk, :, 0] = torch.where(j % 7 == 0, 3e38, 2.9e38 if sign > 0 else 3.2e38)[:, None].to(a.k.dtype) * sign
     a.call()
     weighted(lambda j: (j % 7 == 0).double())
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_attention_one_early_key_that_is_no_number(cuda_mod, t, what):
+    # every later row sees it and is done again: a NaN score ends such a row at once, an
+    # infinite value takes the plain loop's time (a key at a time: 199 ms here)
+    n, heads, d = 4000, 8, 64
+    a = Attn(t, [(n, n)], heads, 2, d, -1, 0, 0, seed=43, interleaved=False)
+    times = []
+    for bad in (False, True):
+        if bad and what == "key":
+            a.k[5, :, 3] = math.nan
+        if bad and what == "value":
+            a.v[5, :, 3] = math.inf
+        a.call()
+        torch.cuda.synchronize()
+        first, last = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        first.record()
+        a.call()
+        last.record()
+        torch.cuda.synchronize()
+        times.append(first.elapsed_time(last))
+    a.check()
+    if what == "key":
+        assert bool(a.out[5:].isnan().all())
+    else:
+        assert bool((a.out[5:, :, 3] == math.inf).all()) and bool(a.out[..., :3].isfinite().all())
+    assert times[1] <= (60 if what == "value" else 10), times
