@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(ROW_THREADS, RowTile<T, DP>::BLOCKS) attn_rows
             w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 1);
             w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 2);
             inv[r] = w.l[r] == 0.0f ? 0.0f : 1.0f / w.l[r];
-            bad[r] = w.l[r] == 0.0f && sees_any(a, pw + r * 8 + (lane >> 2), ln.nk);
+            bad[r] = w.l[r] == 0.0f;  // it sees no key, or scores that overflowed
         }
 #pragma unroll
         for (int n = 0; n < DP / 8; n++)
