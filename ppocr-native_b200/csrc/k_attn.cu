@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(ROW_THREADS, RowTile<T, DP>::BLOCKS) attn_rows
             const uint32_t ks = kv + (it & 1) * 2 * R::K_BYTES, vs = ks + R::K_BYTES;
             const int j0 = kt.first<BK>(it), jend = kt.end(it);
             // nothing here for this warp's rows
-            if ((a.right >= 0 && j0 > pw + 15 + a.right) || (a.left >= 0 && jend <= pw - a.left && j0 >= a.sinks)) continue;
+            if ((a.right >= 0 && j0 > pw + 15 + a.right) || (a.left >= 0 && min(jend, j0 + BK) <= pw - a.left && j0 >= a.sinks)) continue;
             float s[BK / 8][4];
             w.template scores<BK / 8>(s, qw, ks, lane);
             const bool whole = j0 + BK <= jend && (a.right < 0 || j0 + BK - 1 <= pw + a.right) &&
