@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(THREADS) attn_split_kernel(const __grid_consta
                         acc[e] = fmaf(m[x], peer_load(from[x] + uint32_t((r * DP + lane + 32 * e) * 4)), acc[e]);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const int i = int((base + r) / a.share), h = kvh * a.share + int((base + r) % a.share);
-            bool bad = sum == 0.0f && sees_any(a, i + shift, ln.nk);
+            bool bad = sum == 0.0f;  // it sees no key, or scores that overflowed
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 acc[e] *= inv;
