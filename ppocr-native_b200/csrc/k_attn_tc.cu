@@ -192,6 +192,15 @@ struct Tiles {
     }
 };
 
+// The query tiles of a block that gave up behind the one at i0, the plain way (it
+// has some where max_q was too small).
+template <class T>
+__device__ __noinline__ void rest_alone(const AttnArgs &a, int64_t i0) {
+    const Lane ln = read_lane(a, blockIdx.z);
+    while ((i0 += int64_t(gridDim.x) * BQ) < ln.nq)
+        for (int r = threadIdx.x / 32; r < BQ && i0 + r < ln.nq; r += THREADS / 32) row_alone<T>(a, ln, int(i0) + r, blockIdx.y);
+}
+
 // BK keys a tile. Head sizes above 64: 64 keys, 256 columns of tensor memory (two
 // S and P in their places, then 128 of O), two blocks an SM; up to 64: 32 keys,
 // 128 columns (O has 64), four.
@@ -490,7 +499,10 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
         turn += tl.n > 0;
         __syncthreads();  // O is read: the next query tile's product may overwrite it
         fence_after();
-        if (*give_up) break;
+        if (*give_up) {
+            rest_alone<T>(a, i0);
+            break;
+        }
     }
     fence_before();
     __syncthreads();
