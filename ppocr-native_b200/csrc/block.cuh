@@ -44,9 +44,10 @@ void clear_error() noexcept {
 // 0 when every buffer (NULL ones aside) is memory that the current device's
 // kernels may read and write as it is: this device's, managed, or page-locked
 // host memory. Another device's and plain host memory would fault there.
-// About 0.05 us a buffer.
-int check_buffers(const char *what, std::initializer_list<const void *> buffers) noexcept {
+// About 0.05 us a buffer. *local: whether all are this device's own memory.
+int check_buffers(const char *what, std::initializer_list<const void *> buffers, bool *local = nullptr) noexcept {
     int here = 0;
+    if (local) *local = true;
     cudaError_t e = cudaGetDevice(&here);
     for (const void *p : buffers) {
         if (!p || e != cudaSuccess) continue;
@@ -60,6 +61,7 @@ int check_buffers(const char *what, std::initializer_list<const void *> buffers)
         if (at.type == cudaMemoryTypeUnregistered) return refuse(PPOCR_E_ARG, what, "a buffer is not device memory");
         if (at.type == cudaMemoryTypeDevice && at.device != here)
             return refuse(PPOCR_E_ARG, what, "a buffer is another device's than the current one");
+        if (local && at.type != cudaMemoryTypeDevice) *local = false;
     }
     if (e == cudaSuccess) return PPOCR_OK;
     cudaGetLastError();

@@ -218,7 +218,8 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     if (overlap(out, on, q, qn) || (s->kv_rows && (overlap(out, on, k, kn) || overlap(out, on, v, vn))))
         return refuse(PPOCR_E_ARG, me, "out overlaps q, k or v");
 
-    if (const int bad = check_buffers(me, {q, s->kv_rows ? k : nullptr, s->kv_rows ? v : nullptr, out, q_offsets, k_begin, k_len})) return bad;
+    bool local = false;
+    if (const int bad = check_buffers(me, {q, s->kv_rows ? k : nullptr, s->kv_rows ? v : nullptr, out, q_offsets, k_begin, k_len}, &local)) return bad;
 
     AttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.out = out;
@@ -270,8 +271,9 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
         const cudaError_t e = launch_attn_split(a, s->type, max_q, uint32_t(keys), str);
         return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
     }
+    // (tensor copies of the device's own memory alone: no document promises them of the host's)
     bool taken = false;
-    cudaError_t e = launch_attn_tc(a, s->type, max_q, &taken, str);
+    cudaError_t e = local ? launch_attn_tc(a, s->type, max_q, &taken, str) : cudaSuccess;
     if (!taken) e = launch_attn_rows(a, s->type, max_q, str);
     return e == cudaSuccess ? int(PPOCR_OK) : refuse(PPOCR_E_DEVICE, me, cudaGetErrorString(e));
 }

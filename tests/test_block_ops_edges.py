@@ -279,3 +279,44 @@ def test_attention_one_early_key_that_is_no_number(cuda_mod, t, what):
     else:
         assert bool((a.out[5:, :, 3] == math.inf).all()) and bool(a.out[..., :3].isfinite().all())
     assert times[1] <= (60 if what == "value" else 10), times
+
+
+# ---------------------------------------------------------------- buffers
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [40, 64, 128])
+@pytest.mark.parametrize("lens", [[(300, 300), (1, 1), (77, 77)], [(1, 500), (2, 90)]])
+def test_attention_page_locked_buffers(cuda_mod, t, d, lens):
+    a = Attn(t, lens, 4, 2, d, 60, 5, 2, seed=51, interleaved=False, room=510 if lens[0][0] == 1 else 0, pad=2)
+    host = {k: getattr(a, k).contiguous().cpu().pin_memory() for k in ("q", "k", "v", "out", "offsets", "k_begin", "k_len")}
+    strides = {k + "_strides": host[k].stride()[:2] for k in ("q", "k", "v", "out")}
+    cuda.attention_window(a.shape(**strides), *(host[k].data_ptr() for k in ("q", "k", "v", "out", "offsets", "k_begin", "k_len")),
+                          torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    a.out.copy_(host["out"])
+    a.check()
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_norm_and_q4_page_locked_buffers(cuda_mod, t):
+    stream = torch.cuda.current_stream().cuda_stream
+    for c in (256, 101):
+        x, r = (torch.randn(30, c).to(DTYPES[t]).pin_memory() for _ in range(2))
+        s, y = torch.empty_like(x).pin_memory(), torch.empty(30, c, dtype=torch.uint8).pin_memory()
+        gamma, scales = torch.rand(c).pin_memory(), torch.empty(30, 1).pin_memory()
+        cuda.rms_norm_e4m3(cuda.RmsNormShape(t, 30, c, 0, 1e-6), x.data_ptr(), r.data_ptr(), gamma.data_ptr(), s.data_ptr(),
+                           y.data_ptr(), scales.data_ptr(), stream)
+        torch.cuda.synchronize()
+        norm_check(t, x.cuda(), r.cuda(), gamma.cuda(), 1e-6, 0, s.cuda(), y.cuda(), scales.cuda())
+    for m in (1, 2, 16):
+        a = Q4(t, "f32", m, 500, 300, 64, seed=52)
+        a.call()
+        want, dev = a.y.clone(), {k: getattr(a, k) for k in ("x", "w", "scales", "zeros", "bias", "y")}
+        for k, v in dev.items():
+            setattr(a, k, v.cpu().pin_memory())
+        a.y.zero_()
+        a.call()
+        torch.cuda.synchronize()
+        assert torch.equal(a.y.cuda(), want)
