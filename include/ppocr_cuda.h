@@ -183,7 +183,8 @@ int ppocr_db_mask(const float *prob, size_t pixels, float thresh, uint8_t *mask,
  * NULL is the default stream), allocates nothing, keeps nothing, needs no
  * workspace and may run at the same time as any other call, or be captured
  * in a graph. Buffers are the current device's memory, managed or page-locked
- * host memory; plain host memory and another device's are refused. The shapes
+ * host memory; plain host memory and another device's are refused. Tensors may be
+ * columns of one wider buffer, rows of one step side by side. The shapes
  * are read during the call only. Bad arguments return PPOCR_E_ARG and sizes
  * beyond the stated limits PPOCR_E_SIZE before any launch.
  * ---------------------------------------------------------------------- */

@@ -122,6 +122,22 @@ inline bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
     return an && bn && x < y + bn && y < x + an;
 }
 
+// The bytes that rows of a tensor lie in: all of them, and each row's.
+struct Rows {
+    const void *p;
+    uint64_t all, each, step;  // bytes from the first to the last; of a row; from row to row
+};
+
+// True when two tensors' elements may meet: their ranges do, unless rows of one step lie
+// beside one another (columns of one buffer).
+inline bool overlap(const Rows &a, const Rows &b) {
+    if (!overlap(a.p, a.all, b.p, b.all)) return false;
+    if (a.step != b.step || !a.step) return true;
+    const uint64_t from = reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p);
+    const uint64_t off = b.p >= a.p ? from % a.step : (a.step - (0 - from) % a.step) % a.step;
+    return off < a.each || off + b.each > a.step;
+}
+
 // ------------------------------------------------------------ device pieces
 
 __device__ __forceinline__ float to_f32(float v) { return v; }

@@ -215,7 +215,13 @@ extern "C" int ppocr_attention_window(const ppocr_attention_shape *s, const void
     const uint64_t qn = span(s->q_rows, s->q_row, s->heads, s->q_head), on = span(s->q_rows, s->out_row, s->heads, s->out_head);
     const uint64_t kn = span(s->kv_rows, s->k_row, s->kv_heads, s->k_head), vn = span(s->kv_rows, s->v_row, s->kv_heads, s->v_head);
     if (!qn || !on || !kn || !vn) return refuse(PPOCR_E_SIZE, me, "a tensor spans more than 10^15 elements");
-    if (overlap(out, on, q, qn) || (s->kv_rows && (overlap(out, on, k, kn) || overlap(out, on, v, vn))))
+    // rows of all their heads, where these lie side by side
+    const auto rows = [&](const void *p, uint64_t n, uint64_t row, uint64_t heads, uint64_t head) {
+        return Rows{p, n, ((heads - 1) * head + d) * size, row * size};
+    };
+    const Rows outs = rows(out, on, s->out_row, s->heads, s->out_head);
+    if (overlap(outs, rows(q, qn, s->q_row, s->heads, s->q_head)) ||
+        (s->kv_rows && (overlap(outs, rows(k, kn, s->k_row, s->kv_heads, s->k_head)) || overlap(outs, rows(v, vn, s->v_row, s->kv_heads, s->v_head)))))
         return refuse(PPOCR_E_ARG, me, "out overlaps q, k or v");
 
     bool local = false;

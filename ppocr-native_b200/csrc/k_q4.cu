@@ -330,11 +330,15 @@ extern "C" int ppocr_matvec_q4(const ppocr_matvec_q4_shape *s, const void *x, co
     a.w_row = int64_t(s->w_row ? s->w_row : (uint64_t(s->k) + 1) / 2);
     if (a.w_row < (int64_t(s->k) + 1) / 2 || (s->rows > 1 && a.y_row < int64_t(s->n)))
         return refuse(PPOCR_E_ARG, me, "rows of w or y overlap");
-    const uint64_t yn = ((s->rows - 1) * uint64_t(a.y_row) + s->n) * ys, wn = (s->n - 1) * uint64_t(a.w_row) + (uint64_t(s->k) + 1) / 2;
-    if (overlap(y, yn, x, ((s->rows - 1) * uint64_t(a.x_row) + s->k) * xs) || overlap(y, yn, w, wn) ||
-        overlap(y, yn, scales, s->n * groups * ss) || (zeros && overlap(y, yn, zeros, s->n * groups)) ||
-        (bias && overlap(y, yn, bias, s->n * uint64_t(4))) ||
-        (x_scales && overlap(y, yn, x_scales, s->rows * (s->x_group ? groups : 1) * 4)))
+    const auto rows = [](const void *p, uint64_t n, uint64_t row, uint64_t each, uint64_t bytes) {
+        return Rows{p, p ? ((n - 1) * row + each) * bytes : 0, each * bytes, row * bytes};
+    };
+    const Rows yr = rows(y, s->rows, uint64_t(a.y_row), s->n, ys);
+    const uint64_t x_groups = s->x_group ? groups : 1;
+    if (overlap(yr, rows(x, s->rows, uint64_t(a.x_row), s->k, xs)) ||
+        overlap(yr, rows(w, s->n, uint64_t(a.w_row), (uint64_t(s->k) + 1) / 2, 1)) || overlap(yr, rows(scales, s->n, groups, groups, ss)) ||
+        overlap(yr, rows(zeros, s->n, groups, groups, 1)) || overlap(yr, rows(bias, 1, s->n, s->n, 4)) ||
+        overlap(yr, rows(x_scales, s->rows, x_groups, x_groups, 4)))
         return refuse(PPOCR_E_ARG, me, "y overlaps another buffer");
     if (const int bad = check_buffers(me, {x, x_scales, w, scales, zeros, bias, y})) return bad;
     a.scale_type = s->scale_type, a.y_type = s->y_type;

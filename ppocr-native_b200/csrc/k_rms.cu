@@ -472,14 +472,15 @@ extern "C" int ppocr_rms_norm_e4m3(const ppocr_rms_norm_shape *s, const void *x,
     a.group_log2 = s->group == 128 ? 7 : s->group == 64 ? 6 : 5;
     a.eps = s->eps, a.inv_channels = 1.0f / float(c);
     // outputs may meet the inputs only as x or residual updated in place
-    const auto span = [&](int64_t row) { return (s->rows - 1) * uint64_t(row) + c; };
-    const uint64_t xn = span(a.x_row) * size, rn = residual ? span(a.r_row) * size : 0, sn = sum ? span(a.sum_row) * size : 0;
-    const uint64_t yn = span(a.y_row), gn = c * 4, cn = s->rows * uint64_t(a.groups) * 4;
-    const bool over_x = overlap(sum, sn, x, xn) && !(sum == x && a.sum_row == a.x_row);
-    const bool over_r = overlap(sum, sn, residual, rn) && !(sum == residual && a.sum_row == a.r_row);
-    if (over_x || over_r || overlap(sum, sn, gamma, gn) || overlap(sum, sn, y, yn) || overlap(sum, sn, scales, cn) ||
-        overlap(y, yn, x, xn) || overlap(y, yn, residual, rn) || overlap(y, yn, gamma, gn) || overlap(y, yn, scales, cn) ||
-        overlap(scales, cn, x, xn) || overlap(scales, cn, residual, rn) || overlap(scales, cn, gamma, gn))
+    const auto rows = [&](const void *p, int64_t row, uint64_t each, uint64_t bytes) {
+        return Rows{p, p ? ((s->rows - 1) * uint64_t(row) + each) * bytes : 0, each * bytes, uint64_t(row) * bytes};
+    };
+    const Rows xs = rows(x, a.x_row, c, size), rs = rows(residual, a.r_row, c, size), ss = rows(sum, a.sum_row, c, size);
+    const Rows ys = rows(y, a.y_row, c, 1), gs{gamma, c * 4, c * 4, 0}, cs = rows(scales, a.groups, uint64_t(a.groups), 4);
+    const bool over_x = overlap(ss, xs) && !(sum == x && a.sum_row == a.x_row);
+    const bool over_r = overlap(ss, rs) && !(sum == residual && a.sum_row == a.r_row);
+    if (over_x || over_r || overlap(ss, gs) || overlap(ss, ys) || overlap(ss, cs) || overlap(ys, xs) || overlap(ys, rs) ||
+        overlap(ys, gs) || overlap(ys, cs) || overlap(cs, xs) || overlap(cs, rs) || overlap(cs, gs))
         return refuse(PPOCR_E_ARG, me, "an output overlaps another buffer");
     if (const int bad = check_buffers(me, {x, residual, gamma, sum, y, scales})) return bad;
     const auto wide = [&](const void *p, int64_t row) { return !p || (aligned(p, 16) && uint64_t(row) * size % 16 == 0); };

@@ -320,3 +320,74 @@ def test_norm_and_q4_page_locked_buffers(cuda_mod, t):
         a.call()
         torch.cuda.synchronize()
         assert torch.equal(a.y.cuda(), want)
+
+
+def test_columns_of_one_buffer_do_not_overlap():
+    # rows side by side in a wider buffer share no element; one element shared is refused
+    p = 1 << 20
+
+    def outcome(call):
+        with pytest.raises(cuda.PpocrError) as e:
+            call()
+        return "overlap" in str(e.value)
+
+    wide = [(512, 64)] * 4  # q, k, v and out of 2 heads of 64 in rows of 512 elements
+
+    def attention(q, k, v, out, **kw):
+        shape = cuda.AttentionShape(**({"type": "f16", "lanes": 1, "heads": 2, "kv_heads": 2, "head_dim": 64, "q_rows": 9,
+                                        "kv_rows": 9, "scale": 1.0, "q_strides": wide[0], "k_strides": wide[1],
+                                        "v_strides": wide[2], "out_strides": wide[3]} | kw))
+        cuda.attention_window(shape, p + 2 * q, p + 2 * k, p + 2 * v, p + 2 * out, p << 4)
+
+    assert not outcome(lambda: attention(0, 128, 256, 384))
+    assert not outcome(lambda: attention(384, 256, 128, 0))
+    assert outcome(lambda: attention(0, 128, 256, 383)) and outcome(lambda: attention(0, 128, 256, 385))
+    assert outcome(lambda: attention(0, 128, 256, 384, out_strides=(1024, 64)))
+    assert outcome(lambda: attention(0, 512 * 4 + 384 + 64, 256, 384))
+
+    def norm(x, residual, sum, **kw):
+        shape = cuda.RmsNormShape(**({"type": "f16", "rows": 7, "channels": 100, "x_row": 300, "residual_row": 300,
+                                      "sum_row": 300} | kw))
+        cuda.rms_norm_e4m3(shape, p + 2 * x, p + 2 * residual, p << 5, p + 2 * sum, p << 6, p << 7)
+
+    assert not outcome(lambda: norm(0, 100, 200)) and not outcome(lambda: norm(200, 100, 0))
+    assert outcome(lambda: norm(0, 100, 199)) and outcome(lambda: norm(0, 100, 201)) and outcome(lambda: norm(0, 100, 200, sum_row=299))
+
+    def q4(x, y, **kw):
+        shape = cuda.MatvecQ4Shape(**({"x_type": "f16", "y_type": "f16", "scale_type": "f16", "rows": 3, "k": 64, "n": 32,
+                                       "group": 32, "x_row": 96, "y_row": 96} | kw))
+        cuda.matvec_q4(shape, p + 2 * x, None, p << 5, p << 6, None, None, p + 2 * y)
+
+    assert not outcome(lambda: q4(0, 64)) and not outcome(lambda: q4(32, 0)) and not outcome(lambda: q4(96 + 32, 0))
+    assert outcome(lambda: q4(0, 63)) and outcome(lambda: q4(0, 65)) and outcome(lambda: q4(0, 64, y_type="f32"))
+
+
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_outputs_beside_inputs_in_one_buffer(cuda_mod, t):
+    n, h, d, size = 200, 4, 32, torch.finfo(DTYPES[t]).bits // 8
+    a = Attn(t, [(n, n)], h, h, d, 40, 3, 1, seed=61, interleaved=False)
+    rows = torch.full((n, 4 * h, d), 7.0, device="cuda").to(DTYPES[t])
+    rows[:, :h], rows[:, h:2 * h], rows[:, 2 * h:3 * h] = a.q, a.k, a.v
+    a.q, a.k, a.v, a.out = (rows[:, i * h:(i + 1) * h] for i in range(4))
+    before = rows[:, :3 * h].clone()
+    a.call()
+    a.check()
+    assert torch.equal(rows[:, :3 * h], before)
+    c = 120
+    wide = torch.randn(50, 3 * c, device="cuda").to(DTYPES[t])
+    x, r, gamma = wide[:, :c].clone(), wide[:, c:2 * c].clone(), torch.rand(c, device="cuda")
+    y, scales = torch.empty(50, c, dtype=torch.uint8, device="cuda"), torch.empty(50, 1, device="cuda")
+    cuda.rms_norm_e4m3(cuda.RmsNormShape(t, 50, c, 0, 1e-6, 3 * c, 3 * c, 3 * c), wide.data_ptr(), wide.data_ptr() + c * size,
+                       gamma.data_ptr(), wide.data_ptr() + 2 * c * size, y.data_ptr(), scales.data_ptr(),
+                       torch.cuda.current_stream().cuda_stream)
+    norm_check(t, x, r, gamma, 1e-6, 0, wide[:, 2 * c:], y, scales)
+    assert torch.equal(wide[:, :c], x) and torch.equal(wide[:, c:2 * c], r)
+    for m in (1, 8):
+        b = Q4(t, t, m, 256, 96, 32, seed=62)
+        b.call()
+        both = torch.empty(m, 352, device="cuda").to(DTYPES[t])
+        both[:, :256] = b.x
+        want, b.x, b.y = b.y, both, both[:, 256:]
+        b.call(x_row=352, y_row=352)
+        assert torch.equal(both[:, 256:], want)
