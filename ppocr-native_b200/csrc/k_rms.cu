@@ -10,10 +10,10 @@
 // in f32: lane sums, a shuffle tree, then the warps' sums in order (the same
 // order every time), squares that leave its range in sums of scaled values; the next
 // row's loads are out while a row is worked on, and a row costs one barrier. Bound
-// by HBM bytes: 16 384 rows of 4096 in bf16, groups of 128: 84 us, 472 MB at 5.6 TB/s
+// by HBM bytes: 16 384 rows of 4096 in bf16, groups of 128: 83 us, 472 MB at 5.7 TB/s
 // (0.86 of a plain copy's rate; 81 us without the test for squares out of range and
 // what follows it, 184 without the loads ahead). Rows that no vector width divides are
-// read an element at a time, 32 lanes side by side: 1009 rows of 1111 in f16 6.5 us
+// read an element at a time, 32 lanes side by side: 1009 rows of 1111 in f16 6.8 us
 // (7.9 MB, 1.2 us of HBM); 4096 channels so read would take 284 us.
 #include <cuda_fp8.h>
 
@@ -353,10 +353,17 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, at_least<T, TPR, CH, VE
             } else if (mean < 0x1p-75f) {
                 by = TINY, mean = fmaf(apart.x * a.inv_channels * TINY, TINY, apart.z * a.inv_channels) + a.eps * TINY * TINY;
             }
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[c][i] *= by;
+#pragma unroll
+                for (int i = 0; i < (VEC ? 1 : 8); i++) top[c][i] *= by;
+            }
+            all *= by;
         }
         turn ^= 1;
         const float inv = rsqrtf(mean);
-        all *= by;
         float *scales = a.scales + row * a.groups;
         uint8_t *y = a.y + row * a.y_row;
         if (a.group == 0 && channels && t == 0) scales[0] = all * inv * (1.0f / 448.0f);
@@ -364,12 +371,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, at_least<T, TPR, CH, VE
         for (int c = 0; c < CH; c++) {
             const int at = place(c), n = channels - at;
             if (n <= 0) continue;
-            if (by != 1.0f) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[c][i] *= by;
-            }
             if constexpr (VEC) {
-                const float p = (a.group ? top[c][0] * by : all) * inv;
+                const float p = (a.group ? top[c][0] : all) * inv;
                 if (a.group && (at & (a.group - 1)) == 0) scales[at >> a.group_log2] = p * (1.0f / 448.0f);
                 const float f = steps_of(p, inv, v[c]);
                 uint32_t w[2];
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, at_least<T, TPR, CH, VE
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     if (i * 32 >= n) continue;
-                    const float p = (a.group ? top[c][i] * by : all) * inv;
+                    const float p = (a.group ? top[c][i] : all) * inv;
                     if (a.group && lane == 0 && ((at + i * 32) & (a.group - 1)) == 0) scales[(at + i * 32) >> a.group_log2] = p * (1.0f / 448.0f);
                     float one[8] = {v[c][i]};
                     const float f = steps_of(p, inv, one);
