@@ -19,13 +19,14 @@
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (the weights stay below 2^8, their sums in f32), which is rare
-// after the first tile. Bound by the exponentials (16 a cycle and SM) and the
-// products (1280 cycles a 128 keys at head size 128) alike, and by their
-// turns: 8192 queries, 16 heads of 128, window 1024, bf16: 87 to 91 us, 64.7
-// GFLOP at 710 to 740 TFLOP/s (40 us at the library's matrix rate; tensor pipe
-// 45% busy, exponentials 32%, issue 47%), where warp-level products
+// after the first tile: a published way to leave most of a running softmax's
+// corrections out. Bound by the latency of a tile's product, softmax and product one
+// after another, of which two blocks an SM cover about half: 8192 queries, 16 heads of
+// 128, window 1024, bf16: 89 to 96 us from card to card replayed, 101 called one by one,
+// 64.7 GFLOP at 640 to 730 TFLOP/s (40 us at the library's matrix rate; tensor pipe
+// 43% busy, exponentials 41%, issue 39%), where warp-level products
 // (k_attn.cu) take 275. 12 lanes of 1 to 1500 queries, 8 heads of 40, window
-// 257, f16: 34 us and 47. Up to head size 64: tiles of 32 keys and four blocks
+// 257, f16: 35 us and 47. Up to head size 64: tiles of 32 keys and four blocks
 // an SM (34 us, with tiles of 64 and two blocks 37 to 40).
 #include <type_traits>
 

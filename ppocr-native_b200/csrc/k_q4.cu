@@ -53,7 +53,8 @@ __device__ __forceinline__ uint32_t pick(uint32_t w, uint32_t mask, uint32_t mag
 }
 
 // f16: 0x6400 | q is 1024 + q, 0x6400 | q << 4 is 1024 + 16 q; both less their
-// offset are exact.
+// offset are exact (a small integer in the low bits of a float of a fixed exponent: a
+// published way from integers to floats without a conversion).
 template <>
 __device__ __forceinline__ void unpack<__half>(uint32_t w, uint32_t z, uint32_t out[4]) {
     const uint32_t z1 = (0x6400u + z) * 0x10001u;          // 1024 + z, twice
