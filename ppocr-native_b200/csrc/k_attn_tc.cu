@@ -515,6 +515,8 @@ __global__ void __launch_bounds__(THREADS, BK == 64 ? 2 : 4) attn_tc_kernel(cons
 
 bool map_rows(CUtensorMap *map, const void *p, int type, int64_t rows, int64_t row, int heads, int64_t head, int d) {
     const EncodeTiled encode = tensor_map_encoder();
+    // rows or heads that are all the same one: a stride that no document allows
+    if ((heads > 1 && head == 0) || (rows > 1 && row == 0)) return false;
     // a single head's stride is never used, but has to be a valid one
     const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
     const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head : (d + 7) / 8 * 8) * 2, cuuint64_t(rows > 1 ? row : (d + 7) / 8 * 8) * 2};

@@ -281,6 +281,24 @@ def test_attention_one_early_key_that_is_no_number(cuda_mod, t, what):
     assert times[1] <= (60 if what == "value" else 10), times
 
 
+@gpu
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [[(300, 300), (1, 1), (77, 77)], [(1, 500), (2, 90)]])
+def test_attention_broadcast_inputs(cuda_mod, t, lens):
+    # one head, or one row, that stands for all: strides of zero
+    room = 510 if lens[0][0] == 1 else 0
+    for what in ("heads", "rows", "queries"):
+        a = Attn(t, lens, 4, 2, 64, 60, 5, 2, seed=53, interleaved=False, room=room, pad=2)
+        if what == "heads":
+            a.k, a.v = a.k[:, :1].expand(-1, 2, -1), a.v[:, :1].expand(-1, 2, -1)
+        elif what == "rows":
+            a.k, a.v = a.k[:1].expand(a.k.shape[0], -1, -1), a.v[:1].expand(a.v.shape[0], -1, -1)
+        else:
+            a.q = a.q[:1, :1].expand(a.q.shape[0], 4, -1)
+        a.call()
+        a.check()
+
+
 # ---------------------------------------------------------------- buffers
 
 @gpu
